@@ -154,6 +154,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ce4b_quantize_mxfp8": (_i32, [_vp, _vp, _vp, _i32, _i32, _vp]),
     "ce4b_quantize_mxfp8_transpose": (_i32, [_vp, _vp, _vp, _i32, _i32, _vp]),
     "ce4b_mxfp8_gemm": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp]),
+    "ce4b_add_rmsnorm": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _f32, _vp]),
+    "ce4b_add_rmsnorm_mxfp8": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _f32, _vp]),
+    "ce4b_quantize_mxfp4": (_i32, [_vp, _vp, _vp, _i32, _i32, _vp]),
+    "ce4b_dequantize_mxfp4": (_i32, [_vp, _vp, _vp, _i32, _i32, _vp]),
+    "ce4b_mxfp4_linear": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp]),
+    "ce4b_mxfp4_swiglu": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp]),
     "ce4b_dense_block_forward_static": (
         _i32,
         [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _f32, _i32, _vp],

@@ -116,11 +116,86 @@ def residual_add(out: torch.Tensor, residual: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def _check_norm_operands(
+    x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor
+) -> None:
+    _check_bf16_matrix("x", x)
+    _check_bf16_vector("weight", weight, x.shape[1])
+    if residual is not None:
+        _check_bf16_matrix("residual", residual)
+        if residual.shape != x.shape:
+            raise ValueError("residual must match x")
+    if weight.device != x.device or (residual is not None and residual.device != x.device):
+        raise ValueError("residual and weight must be on x's device")
+    _check_extents(x)
+
+
+def _check_extents(tensor: torch.Tensor) -> None:
+    if any(not 1 <= size <= _MAX_EXTENT for size in tensor.shape):
+        raise ValueError(f"extents must be positive and at most {_MAX_EXTENT}")
+
+
+# Extents cross the C ABI as 32-bit integers (with room for padding to whole tiles).
+_MAX_EXTENT = 2**31 - 256
+
+
+def add_rmsnorm_forward(
+    x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float = 1e-6
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The residual addition and the RMSNorm after it in one pass: returns
+    ``s = bf16(x + residual)`` and ``bf16(s * (mean(s^2) + eps)^-1/2 * weight)``.
+
+    What :func:`residual_add` and :func:`rmsnorm_forward` do between two blocks, with the
+    norm rounded once (squares summed in 64 bits), so that a row's result does not depend on
+    the rows around it. With ``residual=None`` it is the norm of ``x``, and ``x`` itself is
+    returned as the sum. BF16 rows of any width.
+    """
+
+    _check_norm_operands(x, residual, weight)
+    out = torch.empty_like(x)
+    total = x if residual is None else torch.empty_like(x)
+    with torch.cuda.device(x.device):
+        _lib.check(
+            _lib.library().ce4b_add_rmsnorm(
+                x.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(),
+                total.data_ptr(), out.data_ptr(), x.shape[0], x.shape[1], eps, _stream(x),
+            )
+        )
+    return total, out
+
+
+def add_rmsnorm_mxfp8(
+    x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float = 1e-6
+) -> tuple[torch.Tensor, Mxfp8Tensor]:
+    """:func:`add_rmsnorm_forward` with the norm as MXFP8: returns the sum and the codes and
+    scales that :func:`quantize_mxfp8` gives for the BF16 norm, bit for bit.
+
+    The width is a multiple of 128; any number of rows (the scale tiles are padded to 128
+    rows with zero bytes, and :func:`mxfp8_gemm` takes such a left operand).
+    """
+
+    _check_norm_operands(x, residual, weight)
+    rows, width = x.shape
+    if width % MXFP8_TILE_SIZE:
+        raise ValueError(f"x must have a multiple of {MXFP8_TILE_SIZE} columns")
+    values = torch.empty_like(x, dtype=torch.float8_e4m3fn)
+    scales = torch.empty(-(-rows // 128), width // 128, 32, 16, dtype=torch.uint8, device=x.device)
+    total = x if residual is None else torch.empty_like(x)
+    with torch.cuda.device(x.device):
+        _lib.check(
+            _lib.library().ce4b_add_rmsnorm_mxfp8(
+                x.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(),
+                total.data_ptr(), values.data_ptr(), scales.data_ptr(), rows, width, eps, _stream(x),
+            )
+        )
+    return total, Mxfp8Tensor(values=values, scales=scales)
+
+
 def dense_block_forward(
     x: torch.Tensor,
     norm_weight: torch.Tensor,
-    gate_up_weight: torch.Tensor,
-    down_weight: torch.Tensor,
+    gate_up_weight: torch.Tensor | Mxfp4Tensor,
+    down_weight: torch.Tensor | Mxfp4Tensor,
     *,
     precision: str,
     eps: float = 1e-6,
@@ -137,13 +212,31 @@ def dense_block_forward(
     gate_up product is a block-scaled GEMM with a BF16 output, SwiGLU runs in BF16, the
     hidden activations and the down weight are quantised and multiplied the same way, and
     the residual is added last; every step is one of this library's kernels.
+
+    ``precision="mxfp4"`` is for search-sized batches, whose time goes to reading weights:
+    the weights are :class:`Mxfp4Tensor` (BF16 ones are quantised per call), the activations
+    stay BF16, and the products are :func:`mxfp4_swiglu` and :func:`mxfp4_linear`.
     """
 
     _check_bf16_matrix("x", x)
     d_model = x.shape[1]
-    if precision not in ("bf16", "mxfp8"):
+    if precision not in ("bf16", "mxfp8", "mxfp4"):
         raise ValueError(f"custom dense kernel does not support precision={precision!r}")
     _check_bf16_vector("norm_weight", norm_weight, d_model)
+    if precision == "mxfp4":
+        gate_up, down = (
+            w if isinstance(w, Mxfp4Tensor) else quantize_mxfp4(w)
+            for w in (gate_up_weight, down_weight)
+        )
+        hidden_dim = down.shape[1]
+        if gate_up.shape != (2 * hidden_dim, d_model):
+            raise ValueError(f"gate_up_weight must have shape [{2 * hidden_dim}, {d_model}]")
+        if down.shape != (d_model, hidden_dim):
+            raise ValueError(f"down_weight must have shape [{d_model}, {hidden_dim}]")
+        _, normalized = add_rmsnorm_forward(x, None, norm_weight, eps)
+        return mxfp4_linear(mxfp4_swiglu(normalized, gate_up), down, residual=x)
+    if isinstance(gate_up_weight, Mxfp4Tensor) or isinstance(down_weight, Mxfp4Tensor):
+        raise ValueError(f"precision={precision!r} takes BF16 weights")
     _check_bf16_matrix("gate_up_weight", gate_up_weight)
     _check_bf16_matrix("down_weight", down_weight)
     hidden_dim = down_weight.shape[1]
@@ -259,6 +352,134 @@ def mxfp8_gemm(left: Mxfp8Tensor, right: Mxfp8Tensor) -> torch.Tensor:
             )
         )
     return out
+
+
+@dataclass(frozen=True, slots=True)
+class Mxfp4Tensor:
+    """An MXFP4 weight [rows, cols]: E2M1 codes, two to a byte with the even column in the low
+    half, and one E8M0 scale per row and 32 columns, in the tiles of :class:`Mxfp8Tensor` with
+    the rows padded to 128."""
+
+    values: torch.Tensor  # uint8 [rows, cols/2]
+    scales: torch.Tensor  # uint8 [ceil(rows/128), cols/128, 32, 16]
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return self.values.shape[0], 2 * self.values.shape[1]
+
+
+def _check_mxfp4(name: str, weight: Mxfp4Tensor, device: torch.device | None = None) -> tuple[int, int]:
+    if not isinstance(weight, Mxfp4Tensor):
+        raise ValueError(f"{name} must be an Mxfp4Tensor")
+    values, scales = weight.values, weight.scales
+    if values.device.type != "cuda" or values.dtype != torch.uint8:
+        raise ValueError(f"{name} values must be a uint8 CUDA tensor")
+    if values.ndim != 2 or not values.is_contiguous():
+        raise ValueError(f"{name} values must be a contiguous matrix")
+    rows, cols = weight.shape
+    _check_extents(values)
+    if cols % MXFP8_TILE_SIZE or cols > _MAX_EXTENT:
+        raise ValueError(f"{name} must have a multiple of {MXFP8_TILE_SIZE} columns")
+    if scales.dtype != torch.uint8 or scales.shape != (-(-rows // 128), cols // 128, 32, 16):
+        raise ValueError(f"{name} scales must be uint8 [{-(-rows // 128)}, {cols // 128}, 32, 16]")
+    if not scales.is_contiguous() or scales.device != values.device:
+        raise ValueError(f"{name} scales must be contiguous and on the values' device")
+    if device is not None and values.device != device:
+        raise ValueError(f"{name} must be on x's device")
+    return rows, cols
+
+
+def quantize_mxfp4(weight: torch.Tensor) -> Mxfp4Tensor:
+    """MXFP4 quantisation of a BF16 weight (columns a multiple of 128, any number of rows).
+
+    Per row and 32 columns, the scale is the smallest power of two (2^-39 at least) that
+    leaves no magnitude over 6, and the codes are E2M1, round to nearest even. A group with
+    a NaN or an infinity stands for NaN.
+    """
+
+    _check_bf16_matrix("weight", weight)
+    _check_extents(weight)
+    rows, cols = weight.shape
+    if cols % MXFP8_TILE_SIZE:
+        raise ValueError(f"weight must have a multiple of {MXFP8_TILE_SIZE} columns")
+    values = torch.empty(rows, cols // 2, dtype=torch.uint8, device=weight.device)
+    scales = torch.empty(-(-rows // 128), cols // 128, 32, 16, dtype=torch.uint8, device=weight.device)
+    with torch.cuda.device(weight.device):
+        _lib.check(
+            _lib.library().ce4b_quantize_mxfp4(
+                weight.data_ptr(), values.data_ptr(), scales.data_ptr(), rows, cols, _stream(weight)
+            )
+        )
+    return Mxfp4Tensor(values=values, scales=scales)
+
+
+def dequantize_mxfp4(weight: Mxfp4Tensor) -> torch.Tensor:
+    """The BF16 matrix that an MXFP4 weight stands for (exact)."""
+
+    rows, cols = _check_mxfp4("weight", weight)
+    values = weight.values
+    out = torch.empty(rows, cols, dtype=torch.bfloat16, device=values.device)
+    with torch.cuda.device(values.device):
+        _lib.check(
+            _lib.library().ce4b_dequantize_mxfp4(
+                values.data_ptr(), weight.scales.data_ptr(), out.data_ptr(), rows, cols, _stream(values)
+            )
+        )
+    return out
+
+
+def mxfp4_linear(
+    x: torch.Tensor, weight: Mxfp4Tensor, *, residual: torch.Tensor | None = None
+) -> torch.Tensor:
+    """``bf16(x @ dequantize(weight).T + residual)`` for a few BF16 rows: FP32 sums, one
+    rounding. Built for search batches (1 to 64 rows), where the time is the weight's bytes;
+    more rows read the weight again for every 64. A NaN or an infinity in a row of ``x``
+    makes that row of the result non-finite."""
+
+    _check_bf16_matrix("x", x)
+    _check_extents(x)
+    n, k = _check_mxfp4("weight", weight, x.device)
+    rows = x.shape[0]
+    if x.shape[1] != k:
+        raise ValueError("MXFP4 product reduction dimensions do not match")
+    if residual is not None:
+        _check_bf16_matrix("residual", residual)
+        if tuple(residual.shape) != (rows, n) or residual.device != x.device:
+            raise ValueError(f"residual must have shape [{rows}, {n}] on x's device")
+    out = torch.empty(rows, n, dtype=torch.bfloat16, device=x.device)
+    with torch.cuda.device(x.device):
+        _lib.check(
+            _lib.library().ce4b_mxfp4_linear(
+                x.data_ptr(), weight.values.data_ptr(), weight.scales.data_ptr(),
+                None if residual is None else residual.data_ptr(), out.data_ptr(), rows, n, k,
+                _stream(x),
+            )
+        )
+    return out
+
+
+def mxfp4_swiglu(x: torch.Tensor, gate_up_weight: Mxfp4Tensor) -> torch.Tensor:
+    """``bf16(silu(g) * u)`` with ``g, u = (x @ dequantize(gate_up_weight).T)`` split in half
+    (gate rows first): the first product of a dense block for a few BF16 rows, FP32 until
+    the one rounding at the end. Rows as in :func:`mxfp4_linear`."""
+
+    _check_bf16_matrix("x", x)
+    _check_extents(x)
+    wide, k = _check_mxfp4("gate_up_weight", gate_up_weight, x.device)
+    rows = x.shape[0]
+    if x.shape[1] != k:
+        raise ValueError("MXFP4 product reduction dimensions do not match")
+    if wide % 2:
+        raise ValueError("gate_up_weight must have an even number of rows")
+    hidden = torch.empty(rows, wide // 2, dtype=torch.bfloat16, device=x.device)
+    with torch.cuda.device(x.device):
+        _lib.check(
+            _lib.library().ce4b_mxfp4_swiglu(
+                x.data_ptr(), gate_up_weight.values.data_ptr(), gate_up_weight.scales.data_ptr(),
+                hidden.data_ptr(), rows, wide // 2, k, _stream(x),
+            )
+        )
+    return hidden
 
 
 EXPERT_COUNT = 64

@@ -592,4 +592,92 @@ int ce4b_mxfp8_gemm(const void* a_codes_dev, const void* a_scales_dev, const voi
   });
 }
 
+// ------------------------------------------------------------------ residual norm, MXFP4
+namespace {
+bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+}  // namespace
+
+int ce4b_add_rmsnorm(const void* x_dev, const void* residual_dev, const void* weight_dev,
+                     void* sum_dev, void* out_dev, int rows, int width, float eps, void* stream) {
+  return guarded([&] {
+    require(x_dev && weight_dev && out_dev, "null pointer");
+    require(residual_dev == nullptr || sum_dev != nullptr, "a residual needs an output for the sum");
+    require(rows >= 1 && width >= 1, "extents must be positive");
+    add_rmsnorm_rows(static_cast<const bf16*>(x_dev), static_cast<const bf16*>(residual_dev),
+                     static_cast<const bf16*>(weight_dev), static_cast<bf16*>(sum_dev),
+                     static_cast<bf16*>(out_dev), nullptr, nullptr, rows, width, eps,
+                     as_stream(stream));
+  });
+}
+
+int ce4b_add_rmsnorm_mxfp8(const void* x_dev, const void* residual_dev, const void* weight_dev,
+                           void* sum_dev, void* codes_dev, void* scales_dev, int rows, int width,
+                           float eps, void* stream) {
+  return guarded([&] {
+    require(x_dev && weight_dev && codes_dev && scales_dev, "null pointer");
+    require(residual_dev == nullptr || sum_dev != nullptr, "a residual needs an output for the sum");
+    require(rows >= 1 && width >= 1, "extents must be positive");
+    require(width % 128 == 0, "MXFP8 rows need a width that is a multiple of 128");
+    require(aligned(codes_dev, 16), "MXFP8 codes must be 16-byte aligned");
+    add_rmsnorm_rows(static_cast<const bf16*>(x_dev), static_cast<const bf16*>(residual_dev),
+                     static_cast<const bf16*>(weight_dev), static_cast<bf16*>(sum_dev), nullptr,
+                     static_cast<uint8_t*>(codes_dev), static_cast<uint8_t*>(scales_dev), rows,
+                     width, eps, as_stream(stream));
+  });
+}
+
+int ce4b_quantize_mxfp4(const void* x_dev, void* codes_dev, void* scales_dev, int rows, int cols,
+                        void* stream) {
+  return guarded([&] {
+    require(x_dev && codes_dev && scales_dev, "null pointer");
+    require(rows >= 1 && cols >= 1, "extents must be positive");
+    require(cols % 128 == 0, "MXFP4 columns must be a multiple of 128");
+    require(aligned(x_dev, 16) && aligned(codes_dev, 16), "MXFP4 buffers must be 16-byte aligned");
+    mx4_quantize(static_cast<const bf16*>(x_dev), static_cast<uint8_t*>(codes_dev),
+                 static_cast<uint8_t*>(scales_dev), rows, cols, as_stream(stream));
+  });
+}
+
+int ce4b_dequantize_mxfp4(const void* codes_dev, const void* scales_dev, void* out_dev, int rows,
+                          int cols, void* stream) {
+  return guarded([&] {
+    require(codes_dev && scales_dev && out_dev, "null pointer");
+    require(rows >= 1 && cols >= 1, "extents must be positive");
+    require(cols % 128 == 0, "MXFP4 columns must be a multiple of 128");
+    require(aligned(codes_dev, 16) && aligned(out_dev, 16), "MXFP4 buffers must be 16-byte aligned");
+    mx4_dequantize(static_cast<const uint8_t*>(codes_dev), static_cast<const uint8_t*>(scales_dev),
+                   static_cast<bf16*>(out_dev), rows, cols, as_stream(stream));
+  });
+}
+
+int ce4b_mxfp4_linear(const void* x_dev, const void* codes_dev, const void* scales_dev,
+                      const void* residual_dev, void* out_dev, int rows, int n, int k,
+                      void* stream) {
+  return guarded([&] {
+    require(x_dev && codes_dev && scales_dev && out_dev, "null pointer");
+    require(rows >= 1 && n >= 1 && k >= 1, "extents must be positive");
+    require(k % 128 == 0, "MXFP4 columns must be a multiple of 128");
+    require(aligned(x_dev, 16) && aligned(codes_dev, 16) && aligned(scales_dev, 16),
+            "MXFP4 operands must be 16-byte aligned");
+    mx4_product(static_cast<const bf16*>(x_dev), static_cast<const uint8_t*>(codes_dev),
+                static_cast<const uint8_t*>(scales_dev), static_cast<const bf16*>(residual_dev),
+                static_cast<bf16*>(out_dev), rows, n, k, false, as_stream(stream));
+  });
+}
+
+int ce4b_mxfp4_swiglu(const void* x_dev, const void* codes_dev, const void* scales_dev,
+                      void* hidden_dev, int rows, int hidden_dim, int k, void* stream) {
+  return guarded([&] {
+    require(x_dev && codes_dev && scales_dev && hidden_dev, "null pointer");
+    require(rows >= 1 && hidden_dim >= 1 && k >= 1, "extents must be positive");
+    require(hidden_dim <= INT32_MAX / 2, "hidden_dim is too large");
+    require(k % 128 == 0, "MXFP4 columns must be a multiple of 128");
+    require(aligned(x_dev, 16) && aligned(codes_dev, 16) && aligned(scales_dev, 16),
+            "MXFP4 operands must be 16-byte aligned");
+    mx4_product(static_cast<const bf16*>(x_dev), static_cast<const uint8_t*>(codes_dev),
+                static_cast<const uint8_t*>(scales_dev), nullptr, static_cast<bf16*>(hidden_dev),
+                rows, hidden_dim, k, true, as_stream(stream));
+  });
+}
+
 }  // extern "C"

@@ -161,6 +161,21 @@ void rmsnorm_rows(const bf16* x, const bf16* w, bf16* out, int rows, int width, 
                   cudaStream_t s);
 void swiglu_rows(const bf16* gate_up, bf16* hidden, int rows, int hidden_dim, cudaStream_t s);
 void residual_add(bf16* out, const bf16* residual, int64_t elements, cudaStream_t s);
+// sum = bf16(x + residual) and its RMSNorm (residual may be null: the norm of x, sum unwritten):
+// BF16 rows in `out`, or, where `codes` is set (width % 128 == 0), MXFP8 codes and scale tiles.
+void add_rmsnorm_rows(const bf16* x, const bf16* residual, const bf16* w, bf16* sum, bf16* out,
+                      uint8_t* codes, uint8_t* scales, int rows, int width, float eps,
+                      cudaStream_t s);
+
+// ---------------------------------------------------------------- MXFP4 weights
+// Codes [rows, cols / 2] and scale tiles [ceil(rows / 128), cols / 128, 512] (cols % 128 == 0).
+void mx4_quantize(const bf16* x, uint8_t* codes, uint8_t* scales, int rows, int cols, cudaStream_t s);
+void mx4_dequantize(const uint8_t* codes, const uint8_t* scales, bf16* out, int rows, int cols,
+                    cudaStream_t s);
+// out [rows, n] = x [rows, k] . W^T (+ residual) over n weight rows, or, with swiglu, over 2n rows
+// (gate rows first) silu(gate) * up.
+void mx4_product(const bf16* x, const uint8_t* codes, const uint8_t* scales, const bf16* residual,
+                 bf16* out, int rows, int n, int k, bool swiglu, cudaStream_t s);
 
 constexpr int kInputPlanes = 112;
 constexpr int kHistoryPlanes = 104;

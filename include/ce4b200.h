@@ -429,6 +429,54 @@ int ce4b_dense_block_forward_static(const void* x_dev, const void* norm_weight_d
                                     void* out_dev, int rows, int d_model, int hidden_dim,
                                     float eps, int precision, void* stream);
 
+/* The residual addition and the RMSNorm after it, one pass: sum = bf16(x + residual) and
+ * out = bf16(sum * (mean(sum^2) + eps)^(-1/2) * w) per row of [rows, width]. The squares are
+ * summed in 64 bits and out is rounded once, so a row's result depends on neither the
+ * launch nor its neighbours. residual_dev may be NULL: the norm of x, and sum_dev is not
+ * written (and may be NULL). sum_dev may be x_dev or residual_dev itself, the buffers
+ * overlap in no other way. Any alignment of the elements; rows, width >= 1. A NaN or an
+ * infinity in a row makes that row's out NaN (0 where the row's other values are finite beside
+ * an infinity). No counterpart in the reference, which adds and normalises in two launches
+ * (kernels/src/sm100/dense.cu:313-348, 379-390). */
+int ce4b_add_rmsnorm(const void* x_dev, const void* residual_dev, const void* weight_dev,
+                     void* sum_dev, void* out_dev, int rows, int width, float eps, void* stream);
+
+/* ce4b_add_rmsnorm with out as the MXFP8 quantisation of its BF16 value, bit for bit what
+ * ce4b_quantize_mxfp8 gives for it: E4M3 codes [rows, width] (16-byte aligned) and E8M0 scales
+ * [ceil(rows/128), width/128, 32, 16]; the scale bytes of rows past the last one are set to 0.
+ * width is a multiple of 128; rows need not be one. */
+int ce4b_add_rmsnorm_mxfp8(const void* x_dev, const void* residual_dev, const void* weight_dev,
+                           void* sum_dev, void* codes_dev, void* scales_dev, int rows, int width,
+                           float eps, void* stream);
+
+/* MXFP4 quantisation of a BF16 weight [rows, cols] (cols a multiple of 128): E2M1 codes
+ * [rows, cols/2], two to a byte with the even column in the low half, and E8M0 scales
+ * [ceil(rows/128), cols/128, 32, 16] in the layout of ce4b_quantize_mxfp8 (padding rows 0).
+ * scale = the smallest power of two, at least 2^-39, that leaves no magnitude of its 32
+ * columns over 6; codes = round-to-nearest-even of x / scale. A group with a NaN or an
+ * infinity gets scale 255, which stands for NaN. x and codes are 16-byte aligned. */
+int ce4b_quantize_mxfp4(const void* x_dev, void* codes_dev, void* scales_dev, int rows, int cols,
+                        void* stream);
+
+/* The BF16 values [rows, cols] that MXFP4 codes and scales stand for (exact where BF16 holds
+ * them: magnitudes below 2^128). codes and out are 16-byte aligned. */
+int ce4b_dequantize_mxfp4(const void* codes_dev, const void* scales_dev, void* out_dev, int rows,
+                          int cols, void* stream);
+
+/* out[rows, n] = bf16(x[rows, k] . W[n, k]^T + residual[rows, n]) with an MXFP4 weight
+ * (FP32 sums, rounded once); residual_dev may be NULL, and may be out_dev itself. For few
+ * rows (search batches): the time goes to reading the 4-bit weight once per 64 rows. x, codes and scales
+ * are 16-byte aligned, k is a multiple of 128. A row of x that holds a NaN or an infinity
+ * gives a row of non-finite values. */
+int ce4b_mxfp4_linear(const void* x_dev, const void* codes_dev, const void* scales_dev,
+                      const void* residual_dev, void* out_dev, int rows, int n, int k,
+                      void* stream);
+
+/* hidden[rows, H] = bf16(silu(g) * u), g and u the products of x [rows, k] with rows 0..H-1
+ * and H..2H-1 of an MXFP4 weight [2H, k] (gate rows first; FP32, rounded once at the end). */
+int ce4b_mxfp4_swiglu(const void* x_dev, const void* codes_dev, const void* scales_dev,
+                      void* hidden_dev, int rows, int hidden_dim, int k, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

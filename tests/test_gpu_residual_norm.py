@@ -1,0 +1,167 @@
+"""GPU tests of the residual addition with its RMSNorm (BF16 and MXFP8 outputs) against the
+formula in 64 bits.
+
+n = s * (mean(s^2) + eps)^-1/2 * w is rounded once from a value that carries over 40 bits, so
+it equals the BF16 rounding of the 64-bit formula except where that value lies within 2^-40
+(relative) of the border between two BF16 neighbours: no element in the sizes tested here is
+expected there, and the comparison is for equality."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+EPS = 1e-6
+
+
+def _inputs(rows: int, width: int, seed: int):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, width, generator=g).bfloat16()
+    residual = (3 * torch.randn(rows, width, generator=g) * torch.exp2(torch.randint(-8, 8, (rows, 1), generator=g).float())).bfloat16()
+    weight = (1 + 0.2 * torch.randn(width, generator=g)).bfloat16()
+    return x.cuda(), residual.cuda(), weight.cuda()
+
+
+def _formula(s: torch.Tensor, weight: torch.Tensor, eps: float = EPS) -> torch.Tensor:
+    eps = float(torch.tensor(eps, dtype=torch.float32))  # eps crosses the ABI in 32 bits
+    v = s.double()
+    n = v / torch.sqrt(v.square().mean(1, keepdim=True) + eps) * weight.double()
+    return _bf16(n)
+
+
+def _bf16(v: torch.Tensor) -> torch.Tensor:
+    """Round 64-bit values to BF16 in one step, through FP32 rounded to odd."""
+
+    f = v.float()
+    back = f.double()
+    bits = f.view(torch.int32)
+    toward_zero = torch.where((back.abs() > v.abs()) & torch.isfinite(back), bits - 1, bits)
+    odd = torch.where(toward_zero.view(torch.float32).double() != v, toward_zero | 1, toward_zero)
+    return torch.where(torch.isfinite(v), odd.view(torch.float32), f).bfloat16()
+
+
+SIZES = [(1, 1), (1, 8), (1, 512), (3, 31), (2, 33), (5, 128), (7, 769), (64, 512), (130, 1000),
+         (9, 2048), (4, 4104), (3, 8192), (2, 8200), (2, 20000), (1, 65536), (1, 70001), (700, 128), (3000, 264)]
+
+
+@pytest.mark.parametrize("rows,width", SIZES)
+def test_add_rmsnorm_forward_is_the_rounded_formula(rows: int, width: int) -> None:
+    from ce4b200 import kernels
+
+    x, residual, weight = _inputs(rows, width, rows + width)
+    total, n = kernels.add_rmsnorm_forward(x, residual, weight)
+    expected = (x.float() + residual.float()).bfloat16()
+    assert torch.equal(total, expected)
+    assert torch.equal(n, _formula(expected, weight))
+
+
+@pytest.mark.parametrize("rows,width", [(1, 512), (5, 129), (33, 2048)])
+def test_without_a_residual_it_is_the_norm_of_x(rows: int, width: int) -> None:
+    from ce4b200 import kernels
+
+    x, _, weight = _inputs(rows, width, 3)
+    total, n = kernels.add_rmsnorm_forward(x, None, weight)
+    assert total is x
+    assert torch.equal(n, _formula(x, weight))
+    # The FP32 operator rounds a value whose error is about 2^-22 of it (sum, root, two
+    # products): it may fall on the other BF16 neighbour, one step of at most 2^-7 away.
+    torch.testing.assert_close(kernels.rmsnorm_forward(x, weight).float(), n.float(), rtol=2.0**-7, atol=0)
+
+
+@pytest.mark.parametrize("rows,width", [(1, 128), (3, 512), (64, 512), (127, 384), (129, 2048), (256, 1024),
+                                        (2, 8192), (1, 16384), (300, 4224)])
+def test_mxfp8_output_equals_quantising_the_bf16_one(rows: int, width: int) -> None:
+    from ce4b200 import kernels
+    from oracle import mxfp8
+
+    x, residual, weight = _inputs(rows, width, rows * width)
+    residual[0, :32] = -x[0, :32]  # an all-zero scale block
+    total, q = kernels.add_rmsnorm_mxfp8(x, residual, weight)
+    plain_total, n = kernels.add_rmsnorm_forward(x, residual, weight)
+    assert torch.equal(total, plain_total)
+    padded = torch.zeros(-(-rows // 128) * 128, width, dtype=torch.bfloat16)
+    padded[:rows] = n.cpu()
+    codes, scales = mxfp8.quantize(padded)
+    assert torch.equal(q.values.view(torch.uint8).cpu(), codes[:rows])
+    got, want = mxfp8.unswizzle_scales(q.scales.cpu()), mxfp8.unswizzle_scales(scales)
+    assert torch.equal(got[:rows], want[:rows])
+    assert not got[rows:].any()
+
+
+def test_a_row_does_not_depend_on_the_batch_or_the_alignment() -> None:
+    from ce4b200 import kernels
+
+    x, residual, weight = _inputs(600, 512, 11)
+    total, n = kernels.add_rmsnorm_forward(x, residual, weight)
+    for r in (0, 17, 599):
+        one_total, one = kernels.add_rmsnorm_forward(x[r:r + 1], residual[r:r + 1], weight)
+        assert torch.equal(one_total[0], total[r]) and torch.equal(one[0], n[r])
+    # The same values at addresses that no wide load may touch.
+    shift = [torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape).copy_(t)
+             for t in (x, residual, weight)]
+    assert shift[0].data_ptr() % 4 == 2
+    odd_total, odd = kernels.add_rmsnorm_forward(*shift)
+    assert torch.equal(odd_total, total) and torch.equal(odd, n)
+    _, q = kernels.add_rmsnorm_mxfp8(x, residual, weight)
+    _, odd_q = kernels.add_rmsnorm_mxfp8(*shift)
+    assert torch.equal(q.values.view(torch.uint8), odd_q.values.view(torch.uint8))
+    assert torch.equal(q.scales, odd_q.scales)
+
+
+def test_special_values_stay_in_their_row() -> None:
+    from ce4b200 import kernels
+
+    x, residual, weight = _inputs(6, 256, 5)
+    x[1], residual[1] = 0, 0
+    x[2, 7] = float("nan")
+    x[3, 9] = float("inf")
+    x[4] = 2.0**100  # squares beyond FP32
+    residual[4] = 2.0**100
+    total, n = kernels.add_rmsnorm_forward(x, residual, weight)
+    clean = [0, 5]
+    assert torch.equal(n[clean], _formula(total[clean], weight))
+    assert not n[1].any()
+    assert n[2].isnan().all()
+    assert n[3, 9].isnan() and not n[3, :9].any() and not n[3, 10:].any()
+    assert torch.equal(n[4], _formula(total[4:5], weight)[0])
+
+
+def test_the_c_entry_writes_the_sum_in_place() -> None:
+    from ce4b200 import _lib, kernels
+
+    x, residual, weight = _inputs(37, 640, 8)
+    total, n = kernels.add_rmsnorm_forward(x, residual, weight)
+    stream = torch.cuda.current_stream().cuda_stream
+    for target in ("x", "residual"):
+        a, b = x.clone(), residual.clone()
+        out = torch.empty_like(x)
+        s = a if target == "x" else b
+        _lib.check(_lib.library().ce4b_add_rmsnorm(
+            a.data_ptr(), b.data_ptr(), weight.data_ptr(), s.data_ptr(), out.data_ptr(), 37, 640, EPS, stream))
+        assert torch.equal(s, total) and torch.equal(out, n)
+
+
+def test_graph_replay_reads_new_inputs() -> None:
+    from ce4b200 import kernels
+
+    x, residual, weight = _inputs(48, 512, 21)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        kernels.add_rmsnorm_mxfp8(x, residual, weight)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        total, n = kernels.add_rmsnorm_forward(x, residual, weight)
+        total8, q = kernels.add_rmsnorm_mxfp8(total, n, weight)
+    x2, residual2, _ = _inputs(48, 512, 22)
+    x.copy_(x2)
+    residual.copy_(residual2)
+    graph.replay()
+    want_total, want_n = kernels.add_rmsnorm_forward(x2, residual2, weight)
+    want_total8, want_q = kernels.add_rmsnorm_mxfp8(want_total, want_n, weight)
+    assert torch.equal(total, want_total) and torch.equal(n, want_n) and torch.equal(total8, want_total8)
+    assert torch.equal(q.values.view(torch.uint8), want_q.values.view(torch.uint8))
+    assert torch.equal(q.scales, want_q.scales)
