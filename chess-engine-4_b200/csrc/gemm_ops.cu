@@ -10,6 +10,7 @@
 #include "forward.cuh"
 #include "gemm.cuh"
 #include "internal.h"
+#include "launch.cuh"
 
 namespace ce4b {
 
@@ -34,21 +35,6 @@ EncodeTiledFn encode_fn() {
   });
   if (fn == nullptr) fail(CE4B_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   return fn;
-}
-
-// Opt each kernel instantiation into the dynamic shared memory it needs, once per device.
-template <class K>
-void ensure_smem(K kernel, int bytes) {
-  static std::mutex mu;
-  static std::set<std::pair<int, const void*>> done;
-  int dev = 0;
-  check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
-  const auto key = std::make_pair(dev, reinterpret_cast<const void*>(kernel));
-  std::lock_guard<std::mutex> lock(mu);
-  if (done.count(key)) return;
-  check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
-             "cudaFuncSetAttribute(max dynamic smem)");
-  done.insert(key);
 }
 
 // Clusters of `cluster` CTAs of `kernel` that fit on the device at once (cached).
@@ -78,33 +64,6 @@ int max_active_clusters(K kernel, int threads, int smem, int cluster) {
   require(n >= 1, "no cluster of " + std::to_string(cluster) + " CTAs fits on this device");
   cache.emplace(key, n);
   return n;
-}
-
-template <class K, class... Args>
-void launch(K kernel, dim3 grid, int threads, int smem, int cluster_x, cudaStream_t s,
-            Args... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
-  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
-  cfg.stream = s;
-  // Every GEMM kernel waits for its predecessor (grid_dependency_wait) before touching
-  // global memory, so it may be launched programmatically: its CTAs take SMs as the
-  // previous kernel's CTAs leave and run their prologue under that kernel's tail.
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  unsigned n_attr = 1;
-  if (cluster_x > 0) {
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster_x);
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    n_attr = 2;
-  }
-  cfg.attrs = attr;
-  cfg.numAttrs = n_attr;
-  check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), "gemm launch");
 }
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
@@ -164,8 +123,9 @@ CUtensorMap make_tmap_bf16(const void* ptr, uint64_t rows, uint64_t cols, uint64
   return map;
 }
 
-CUtensorMap make_tmap_u8(const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld_bytes,
-                         uint32_t box_rows) {
+namespace {
+CUtensorMap encode_u8(const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld_bytes, uint32_t box_cols,
+                      uint32_t box_rows, CUtensorMapSwizzle swizzle) {
   require(ptr != nullptr, "tensor map: null pointer");
   require((reinterpret_cast<uintptr_t>(ptr) & 15u) == 0, "tensor map: base not 16-byte aligned");
   require(ld_bytes % 16 == 0, "tensor map: row stride not a multiple of 16 bytes");
@@ -173,14 +133,25 @@ CUtensorMap make_tmap_u8(const void* ptr, uint64_t rows, uint64_t cols, uint64_t
   CUtensorMap map;
   const cuuint64_t gdim[2] = {cols, rows};
   const cuuint64_t gstride[1] = {ld_bytes};
-  const cuuint32_t box[2] = {128, box_rows};
+  const cuuint32_t box[2] = {box_cols, box_rows};
   const cuuint32_t estride[2] = {1, 1};
   const CUresult r = encode_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr),
                                  gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                 swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) fail(CE4B_ERR_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string(r));
   return map;
+}
+}  // namespace
+
+CUtensorMap make_tmap_u8(const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld_bytes,
+                         uint32_t box_rows) {
+  return encode_u8(ptr, rows, cols, ld_bytes, 128, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+CUtensorMap make_tmap_u8_sw64(const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld_bytes,
+                              uint32_t box_rows) {
+  return encode_u8(ptr, rows, cols, ld_bytes, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 // ------------------------------------------------------------------ MXFP8 GEMMs

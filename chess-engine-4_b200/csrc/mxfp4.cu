@@ -1,4 +1,4 @@
-// MXFP4 weights (kernel-op API quantize_mxfp4, dequantize_mxfp4, mxfp4_linear, mxfp4_swiglu):
+// MXFP4 weights (kernel-op API quantize_mxfp4, dequantize_mxfp4):
 // E2M1 codes, two to a byte with the even column in the low half, and one E8M0 scale per row
 // and 32 columns in the scale tiles of MXFP8 tensors (rows padded to 128).
 #include <cuda_fp4.h>
@@ -82,49 +82,6 @@ __global__ void mx4_dequantize_kernel(const uint8_t* __restrict__ codes,
   }
 }
 
-constexpr int kRowsPerPass = 8;
-
-// One warp per output column and 8 activation rows; FP32 sums.
-template <bool SWIGLU>
-__global__ void mx4_product_kernel(const bf16* __restrict__ x, const uint8_t* __restrict__ codes,
-                                   const uint8_t* __restrict__ scales,
-                                   const bf16* residual, bf16* out, int rows, int n, int k) {
-  const int col = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-  const int lane = threadIdx.x & 31;
-  const int r0 = blockIdx.y * kRowsPerPass;
-  if (col >= n) return;
-  float acc[2][kRowsPerPass] = {};
-#pragma unroll
-  for (int h = 0; h < (SWIGLU ? 2 : 1); ++h) {
-    const int row = col + h * n;
-    for (int g = 0; g < k / 32; ++g) {
-      const uint32_t byte = codes[static_cast<size_t>(row) * (k / 2) + g * 16 + lane / 2];
-      const float w = mx4_value(lane & 1 ? byte >> 4 : byte & 15u) *
-                      mx4_scale(scales[mx_scale_offset(row, g, k / 128)]);
-#pragma unroll
-      for (int r = 0; r < kRowsPerPass; ++r) {
-        if (r0 + r < rows) {
-          acc[h][r] = fmaf(w, __bfloat162float(x[static_cast<size_t>(r0 + r) * k + g * 32 + lane]), acc[h][r]);
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < kRowsPerPass; ++r) {
-    for (int o = 16; o > 0; o >>= 1) {
-      acc[0][r] += __shfl_xor_sync(0xffffffffu, acc[0][r], o);
-      if (SWIGLU) acc[1][r] += __shfl_xor_sync(0xffffffffu, acc[1][r], o);
-    }
-    if (lane == 0 && r0 + r < rows) {
-      const size_t at = static_cast<size_t>(r0 + r) * n + col;
-      float v = acc[0][r];
-      if (SWIGLU) v = v / (1.0f + expf(-v)) * acc[1][r];
-      if (residual != nullptr) v += __bfloat162float(residual[at]);
-      out[at] = __float2bfloat16_rn(v);
-    }
-  }
-}
-
 int grid_for(int64_t work, int threads) {
   return static_cast<int>(std::min<int64_t>((work + threads - 1) / threads, static_cast<int64_t>(sm_count()) * 16));
 }
@@ -142,17 +99,6 @@ void mx4_dequantize(const uint8_t* codes, const uint8_t* scales, bf16* out, int 
   const int64_t work = static_cast<int64_t>(rows) * (cols / 32);
   mx4_dequantize_kernel<<<grid_for(work, 256), 256, 0, s>>>(codes, scales, out, rows, cols);
   check_cuda(cudaGetLastError(), "dequantize_mxfp4 launch");
-}
-
-void mx4_product(const bf16* x, const uint8_t* codes, const uint8_t* scales, const bf16* residual,
-                 bf16* out, int rows, int n, int k, bool swiglu, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>((n + 7) / 8), static_cast<unsigned>((rows + kRowsPerPass - 1) / kRowsPerPass));
-  if (swiglu) {
-    mx4_product_kernel<true><<<grid, 256, 0, s>>>(x, codes, scales, nullptr, out, rows, n, k);
-  } else {
-    mx4_product_kernel<false><<<grid, 256, 0, s>>>(x, codes, scales, residual, out, rows, n, k);
-  }
-  check_cuda(cudaGetLastError(), "mxfp4 product launch");
 }
 
 }  // namespace ce4b

@@ -9,8 +9,8 @@ namespace ce4b {
 
 namespace {
 
-// n is the correctly rounded BF16 of its formula: the squares (exact in 64 bits) are summed in
-// 64 bits and the factor (mean + eps)^(-1/2) is kept as an FP32 pair hi + lo, so that a row's
+// n is the BF16 rounding of the formula's FP32 value: the squares (exact in 64 bits) are summed
+// in 64 bits and the factor (mean + eps)^(-1/2) is kept as an FP32 pair hi + lo, so that a row's
 // result does not depend on the order of its sum, on the launch shape or on the row's
 // neighbours. Every form of the operator gives the same n, and the MXFP8 form quantises
 // exactly that value.
@@ -26,17 +26,14 @@ __device__ __forceinline__ RowScale row_scale(double sum, double inv_width, floa
   return r;
 }
 
-// bf16(s * (hi + lo) * w), rounded once: q is the FP32 rounding of the product and e the rest.
-// Rounding q gives the wrong neighbour only where q sits on the border between two BF16
-// values (its low half is 0x8000) and the rest moves the product off it.
+// s * (hi + lo) * w: q is the FP32 rounding of the product and e the rest, so that q + e is the
+// product rounded to FP32 once (about 2^-46 of it is lost before). An overflowing q has no rest.
 __device__ __forceinline__ float scale_round(float s, float w, const RowScale& f) {
   const float t = s * f.hi;
   const float te = fmaf(s, f.lo, fmaf(s, f.hi, -t));
   const float q = t * w;
   const float e = fmaf(te, w, fmaf(t, w, -q));
-  uint32_t b = __float_as_uint(q);
-  if ((b & 0xFFFFu) == 0x8000u && e != 0.0f) b = (e > 0.0f) == (q > 0.0f) ? b + 1u : b - 1u;
-  return bf16_round(__uint_as_float(b));
+  return bf16_round(fabsf(q) <= 3.0e38f ? q + e : q);
 }
 
 __device__ __forceinline__ double block_sum(double v) {

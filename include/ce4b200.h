@@ -431,8 +431,8 @@ int ce4b_dense_block_forward_static(const void* x_dev, const void* norm_weight_d
 
 /* The residual addition and the RMSNorm after it, one pass: sum = bf16(x + residual) and
  * out = bf16(sum * (mean(sum^2) + eps)^(-1/2) * w) per row of [rows, width]. The squares are
- * summed in 64 bits and out is rounded once, so a row's result depends on neither the
- * launch nor its neighbours. residual_dev may be NULL: the norm of x, and sum_dev is not
+ * summed in 64 bits and out is rounded from the formula's FP32 value, so a row's result
+ * depends on neither the launch nor its neighbours. residual_dev may be NULL: the norm of x, and sum_dev is not
  * written (and may be NULL). sum_dev may be x_dev or residual_dev itself, the buffers
  * overlap in no other way. Any alignment of the elements; rows, width >= 1. A NaN or an
  * infinity in a row makes that row's out NaN (0 where the row's other values are finite beside

@@ -1,10 +1,10 @@
 """GPU tests of the residual addition with its RMSNorm (BF16 and MXFP8 outputs) against the
 formula in 64 bits.
 
-n = s * (mean(s^2) + eps)^-1/2 * w is rounded once from a value that carries over 40 bits, so
-it equals the BF16 rounding of the 64-bit formula except where that value lies within 2^-40
-(relative) of the border between two BF16 neighbours: no element in the sizes tested here is
-expected there, and the comparison is for equality."""
+n = s * (mean(s^2) + eps)^-1/2 * w is computed to over 40 bits, rounded to FP32 and then to
+BF16, as a conversion from 64 bits does. It equals the formula rounded that way except where
+the 64-bit value lies within 2^-40 (relative) of a border: no element in the sizes tested
+here is expected there, and the comparison is for equality."""
 
 from __future__ import annotations
 
@@ -28,18 +28,7 @@ def _formula(s: torch.Tensor, weight: torch.Tensor, eps: float = EPS) -> torch.T
     eps = float(torch.tensor(eps, dtype=torch.float32))  # eps crosses the ABI in 32 bits
     v = s.double()
     n = v / torch.sqrt(v.square().mean(1, keepdim=True) + eps) * weight.double()
-    return _bf16(n)
-
-
-def _bf16(v: torch.Tensor) -> torch.Tensor:
-    """Round 64-bit values to BF16 in one step, through FP32 rounded to odd."""
-
-    f = v.float()
-    back = f.double()
-    bits = f.view(torch.int32)
-    toward_zero = torch.where((back.abs() > v.abs()) & torch.isfinite(back), bits - 1, bits)
-    odd = torch.where(toward_zero.view(torch.float32).double() != v, toward_zero | 1, toward_zero)
-    return torch.where(torch.isfinite(v), odd.view(torch.float32), f).bfloat16()
+    return n.float().bfloat16()
 
 
 SIZES = [(1, 1), (1, 8), (1, 512), (3, 31), (2, 33), (5, 128), (7, 769), (64, 512), (130, 1000),
