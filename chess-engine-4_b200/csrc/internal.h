@@ -179,6 +179,10 @@ void mx4_dequantize(const uint8_t* codes, const uint8_t* scales, bf16* out, int 
 // (gate rows first) silu(gate) * up.
 void mx4_product(const bf16* x, const uint8_t* codes, const uint8_t* scales, const bf16* residual,
                  bf16* out, int rows, int n, int k, bool swiglu, cudaStream_t s);
+// Its form for many rows, on tcgen05 MMAs.
+void mx4_product_tc(const bf16* x, const uint8_t* codes, const uint8_t* scales,
+                    const bf16* residual, bf16* out, int rows, int n, int k, bool swiglu,
+                    cudaStream_t s);
 
 constexpr int kInputPlanes = 112;
 constexpr int kHistoryPlanes = 104;

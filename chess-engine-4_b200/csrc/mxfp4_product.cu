@@ -20,6 +20,7 @@
 
 #include "internal.h"
 #include "launch.cuh"
+#include "mxfp4.cuh"
 #include "ptx.cuh"
 
 namespace ce4b {
@@ -51,34 +52,21 @@ struct ProductSmem {
   static_assert(kBytes <= 113 * 1024, "two CTAs must fit on an SM");
 };
 
-// The 32 codes of one group (16 bytes) as 16 registers of two BF16 values each, in order.
-// A table of the eight scaled magnitudes is split into low and high bytes; a byte permute
-// looks up four codes at once (its selector nibbles are the codes themselves), the sign bits
-// are merged into the high bytes, and two more permutes interleave the halves.
+// The 32 codes of one group (16 bytes) as 16 registers of two BF16 values each.
 __device__ __forceinline__ void expand_group(const uint4& q, uint32_t scale, uint32_t* out) {
-  uint32_t f = scale * 0x00800080u;                  // 2^(scale - 127), twice
-  if (scale == 0u) f = 0x00400040u;                  // 2^-127 is subnormal
-  if (scale == 255u) f = 0x7FFF7FFFu;                // NaN
-  const __nv_bfloat162 f2 = *reinterpret_cast<const __nv_bfloat162*>(&f);
-  auto pair = [&](uint32_t c) {
-    const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&c), f2);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  };
-  const uint32_t p0 = pair(0x3F000000u), p1 = pair(0x3FC03F80u);  // 0, 0.5, 1, 1.5
-  const uint32_t p2 = pair(0x40404000u), p3 = pair(0x40C04080u);  // 2, 3, 4, 6
-  const uint32_t lo0 = prmt(p0, p1, 0x6420u), lo1 = prmt(p2, p3, 0x6420u);
-  const uint32_t hi0 = prmt(p0, p1, 0x7531u), hi1 = prmt(p2, p3, 0x7531u);
+  const uint32_t f = mx4_factor(scale);
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t m = w[i] & 0x77777777u, m4 = m >> 16, u = w[i] << 4;
-    const uint32_t l0 = prmt(lo0, lo1, m), l1 = prmt(lo0, lo1, m4);
-    const uint32_t h0 = prmt(hi0, hi1, m) | (prmt(u, w[i], 0x5140u) & 0x80808080u);
-    const uint32_t h1 = prmt(hi0, hi1, m4) | (prmt(u, w[i], 0x7362u) & 0x80808080u);
-    out[4 * i] = prmt(l0, h0, 0x5140u);
-    out[4 * i + 1] = prmt(l0, h0, 0x7362u);
-    out[4 * i + 2] = prmt(l1, h1, 0x5140u);
-    out[4 * i + 3] = prmt(l1, h1, 0x7362u);
+    uint32_t v[4];
+    mx4_expand(w[i], f, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[4 * i + j] = v[j];
+  }
+  if (__any_sync(0xffffffffu, scale > 128u)) {
+    const uint32_t g = mx4_factor2(scale);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) out[i] = mul_bf16x2(out[i], g);
   }
 }
 
@@ -121,7 +109,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_init(empty_bar(s), 1);
     }
     for (int a = 0; a < kABuffers; ++a) {
-      mbar_init(afull_bar(a), kExpandWarps);
+      mbar_init(afull_bar(a), 4);
       mbar_init(aempty_bar(a), 1);
     }
     mbar_init(done_bar, 1);
@@ -205,7 +193,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     __syncwarp();
   } else {
-    const int half = (warp - 2) / 4;                // which 64 of a stage's 128 columns
+    // Four warps cover the 128 lanes; the first four expand the even stages, the others the odd.
+    const int turn = (warp - 2) / 4;
     const int r = (warp & 3) * 32 + lane;           // weight row in the tile = lane of TMEM
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     // Where the row's four scale bytes of a K block lie in the stage's scale tiles.
@@ -217,31 +206,42 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     const uint32_t sf_off = L::kCodeBytes + L::kXBytes + area * 512 + (tile_row % 32) * 16 + (tile_row / 32) * 4;
     const uint32_t swz = (r >> 1) & 3;
-    int it = 0;
-    for (int kb = kb0; kb < kb1; ++kb, ++it) {
+    for (int it = turn; it < kb1 - kb0; it += 2) {
       const int s = it % NS, a = it % kABuffers;
-      if (!mbar_wait(full_bar(s), (it / NS) & 1) ||
-          !mbar_wait(aempty_bar(a), ((it / kABuffers) & 1) ^ 1)) {
+      if (!mbar_wait(full_bar(s), (it / NS) & 1)) {
+        record_error(err, kErrTimeoutEpilogue);
+        break;
+      }
+      const uint32_t stage = base + s * L::kStageBytes;
+      const uint32_t row = stage + r * 64;
+#pragma unroll
+      for (int i = 0; i < R * 16 / 128; ++i) {
+        const uint32_t at = stage + L::kCodeBytes + (i * 128 + r) * 16;
+        st_shared_v4(at, permute_x(ld_shared_v4(at)));
+      }
+      fence_proxy_async_smem();
+      const uint32_t sf = __float_as_uint(ld_shared_f32(stage + sf_off));
+      if (!mbar_wait(aempty_bar(a), ((it / kABuffers) & 1) ^ 1)) {
         record_error(err, kErrTimeoutEpilogue);
         break;
       }
       tc_fence_after();
-      const uint32_t stage = base + s * L::kStageBytes;
-      const uint32_t row = stage + r * 64;
-      const uint4 q0 = ld_shared_v4(row + (((2u * half) ^ swz) << 4));
-      const uint4 q1 = ld_shared_v4(row + (((2u * half + 1u) ^ swz) << 4));
-      const uint32_t sf = __float_as_uint(ld_shared_f32(stage + sf_off)) >> (16 * half);
-      uint32_t v[32];
-      expand_group(q0, sf & 255u, v);
-      expand_group(q1, (sf >> 8) & 255u, v + 16);
-      tmem_st32(tmem + lane_base + kACol + 64u * a + 32u * half, v);
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) {
+        const uint4 q0 = ld_shared_v4(row + (((2u * h) ^ swz) << 4));
+        const uint4 q1 = ld_shared_v4(row + (((2u * h + 1u) ^ swz) << 4));
+        uint32_t v[32];
+        expand_group(q0, (sf >> (16u * h)) & 255u, v);
+        expand_group(q1, (sf >> (16u * h + 8u)) & 255u, v + 16);
+        tmem_st32(tmem + lane_base + kACol + 64u * a + 32u * h, v);
+      }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(afull_bar(a));
     }
     // Partial sums [activation row][weight row] in FP32, over the ring.
-    if (half == 0) {
+    if (turn == 0) {
       if (!mbar_wait(done_bar, 0)) record_error(err, kErrTimeoutEpilogue);
       tc_fence_after();
       float* part = reinterpret_cast<float*>(smem);
@@ -294,6 +294,22 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (split > 1) cluster_sync_all();  // a peer may still read this CTA's sums
 }
 
+// CTAs per row tile. The CTAs of an SM share its issue slots, so a launch takes as long as the
+// SM with the most of them: ceil(tiles * split / SMs) times kblocks / split ring stages and a
+// fixed part (launch, tensor memory, pipeline fill, join) worth about kFixed stages.
+int choose_split(int tiles, int kblocks) {
+  constexpr int kFixed = 3;
+  const int sms = sm_count();
+  int best = 1;
+  int64_t best_cost = INT64_MAX;
+  for (int split = 1; split <= std::min(kMaxSplit, kblocks); ++split) {
+    const int64_t turns = (static_cast<int64_t>(tiles) * split + sms - 1) / sms;
+    const int64_t cost = turns * ((kblocks + split - 1) / split + kFixed);
+    if (cost < best_cost) best_cost = cost, best = split;
+  }
+  return best;
+}
+
 template <int R, bool SWIGLU>
 void launch_product(const bf16* x, const uint8_t* codes, const uint8_t* scales,
                     const bf16* residual, bf16* out, int rows, int n, int k, cudaStream_t s) {
@@ -305,8 +321,7 @@ void launch_product(const bf16* x, const uint8_t* codes, const uint8_t* scales,
   const CUtensorMap tc = make_tmap_u8_sw64(codes, wide, k / 2, k / 2, kCols);
   const CUtensorMap tx = make_tmap_bf16(x, rows, k, k, R);
   const int tiles = (n + kCols - 1) / kCols, kblocks = k / kKB;
-  int split = 1;
-  while (split < kMaxSplit && 2 * split <= kblocks && tiles * 2 * split <= 2 * sm_count()) split *= 2;
+  const int split = choose_split(tiles * ((rows + R - 1) / R), kblocks);
   const dim3 grid(static_cast<unsigned>(tiles * split), static_cast<unsigned>((rows + R - 1) / R));
   launch(kernel, grid, kThreads, L::kBytes, split > 1 ? split : 0, s, tc, tx, scales, residual, out,
          rows, n, kblocks, split, device_error_word());
@@ -314,20 +329,15 @@ void launch_product(const bf16* x, const uint8_t* codes, const uint8_t* scales,
 
 }  // namespace
 
-void mx4_product(const bf16* x, const uint8_t* codes, const uint8_t* scales, const bf16* residual,
-                 bf16* out, int rows, int n, int k, bool swiglu, cudaStream_t s) {
+void mx4_product_tc(const bf16* x, const uint8_t* codes, const uint8_t* scales,
+                    const bf16* residual, bf16* out, int rows, int n, int k, bool swiglu,
+                    cudaStream_t s) {
   if (swiglu) {
-    if (rows <= 16) {
-      launch_product<16, true>(x, codes, scales, nullptr, out, rows, n, k, s);
-    } else if (rows <= 32) {
+    if (rows <= 32) {
       launch_product<32, true>(x, codes, scales, nullptr, out, rows, n, k, s);
     } else {
       launch_product<64, true>(x, codes, scales, nullptr, out, rows, n, k, s);
     }
-    return;
-  }
-  if (rows <= 16) {
-    launch_product<16, false>(x, codes, scales, residual, out, rows, n, k, s);
   } else if (rows <= 32) {
     launch_product<32, false>(x, codes, scales, residual, out, rows, n, k, s);
   } else {
