@@ -116,18 +116,8 @@ def residual_add(out: torch.Tensor, residual: torch.Tensor) -> torch.Tensor:
     return out
 
 
-def _check_norm_operands(
-    x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor
-) -> None:
-    _check_bf16_matrix("x", x)
-    _check_bf16_vector("weight", weight, x.shape[1])
-    if residual is not None:
-        _check_bf16_matrix("residual", residual)
-        if residual.shape != x.shape:
-            raise ValueError("residual must match x")
-    if weight.device != x.device or (residual is not None and residual.device != x.device):
-        raise ValueError("residual and weight must be on x's device")
-    _check_extents(x)
+# Extents cross the C ABI as 32-bit integers (with room for padding to whole tiles).
+_MAX_EXTENT = 2**31 - 256
 
 
 def _check_extents(tensor: torch.Tensor) -> None:
@@ -135,8 +125,49 @@ def _check_extents(tensor: torch.Tensor) -> None:
         raise ValueError(f"extents must be positive and at most {_MAX_EXTENT}")
 
 
-# Extents cross the C ABI as 32-bit integers (with room for padding to whole tiles).
-_MAX_EXTENT = 2**31 - 256
+# The operators below are called once per layer on batches of a few rows, where the host's
+# time per call is the call's time: what is as it should be is recognised by a few cheap
+# tests, and the checks that word an error run only if one of those fails.
+def _need_bf16_matrix(name: str, tensor: torch.Tensor) -> None:
+    if not (tensor.is_cuda and tensor.dtype is torch.bfloat16 and tensor.dim() == 2 and tensor.is_contiguous()):
+        _check_bf16_matrix(name, tensor)
+    rows, cols = tensor.shape
+    if not (1 <= rows <= _MAX_EXTENT and 1 <= cols <= _MAX_EXTENT):
+        _check_extents(tensor)
+
+
+def _same_device(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.get_device() == b.get_device() if a.is_cuda and b.is_cuda else a.device == b.device
+
+
+def _call(name: str, tensor: torch.Tensor, *args: object) -> None:
+    """Call a C entry (its last argument is the stream) on `tensor`'s device and stream."""
+
+    fn = getattr(_lib.library(), name)
+    index = tensor.get_device()
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status)
+
+
+def _check_norm_operands(
+    x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor
+) -> None:
+    _need_bf16_matrix("x", x)
+    if residual is not None:
+        _need_bf16_matrix("residual", residual)
+        if residual.shape != x.shape:
+            raise ValueError("residual must match x")
+        if not _same_device(residual, x):
+            raise ValueError("residual must be on x's device")
+    if not (weight.is_cuda and weight.dtype is torch.bfloat16 and weight.shape == x.shape[1:] and weight.is_contiguous()):
+        _check_bf16_vector("weight", weight, x.shape[1])
+    if not _same_device(weight, x):
+        raise ValueError("weight must be on x's device")
 
 
 def add_rmsnorm_forward(
@@ -154,13 +185,9 @@ def add_rmsnorm_forward(
     _check_norm_operands(x, residual, weight)
     out = torch.empty_like(x)
     total = x if residual is None else torch.empty_like(x)
-    with torch.cuda.device(x.device):
-        _lib.check(
-            _lib.library().ce4b_add_rmsnorm(
-                x.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(),
-                total.data_ptr(), out.data_ptr(), x.shape[0], x.shape[1], eps, _stream(x),
-            )
-        )
+    _call(
+        "ce4b_add_rmsnorm", x, x.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(), total.data_ptr(), out.data_ptr(), x.shape[0], x.shape[1], eps,
+    )
     return total, out
 
 
@@ -181,13 +208,9 @@ def add_rmsnorm_mxfp8(
     values = torch.empty_like(x, dtype=torch.float8_e4m3fn)
     scales = torch.empty(-(-rows // 128), width // 128, 32, 16, dtype=torch.uint8, device=x.device)
     total = x if residual is None else torch.empty_like(x)
-    with torch.cuda.device(x.device):
-        _lib.check(
-            _lib.library().ce4b_add_rmsnorm_mxfp8(
-                x.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(),
-                total.data_ptr(), values.data_ptr(), scales.data_ptr(), rows, width, eps, _stream(x),
-            )
-        )
+    _call(
+        "ce4b_add_rmsnorm_mxfp8", x, x.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(), total.data_ptr(), values.data_ptr(), scales.data_ptr(), rows, width, eps,
+    )
     return total, Mxfp8Tensor(values=values, scales=scales)
 
 
@@ -368,23 +391,26 @@ class Mxfp4Tensor:
         return self.values.shape[0], 2 * self.values.shape[1]
 
 
-def _check_mxfp4(name: str, weight: Mxfp4Tensor, device: torch.device | None = None) -> tuple[int, int]:
+def _need_mxfp4(name: str, weight: Mxfp4Tensor, x: torch.Tensor | None = None) -> tuple[int, int]:
     if not isinstance(weight, Mxfp4Tensor):
         raise ValueError(f"{name} must be an Mxfp4Tensor")
     values, scales = weight.values, weight.scales
-    if values.device.type != "cuda" or values.dtype != torch.uint8:
-        raise ValueError(f"{name} values must be a uint8 CUDA tensor")
-    if values.ndim != 2 or not values.is_contiguous():
-        raise ValueError(f"{name} values must be a contiguous matrix")
-    rows, cols = weight.shape
-    _check_extents(values)
-    if cols % MXFP8_TILE_SIZE or cols > _MAX_EXTENT:
+    if not (values.is_cuda and values.dtype is torch.uint8 and values.dim() == 2 and values.is_contiguous()):
+        if values.device.type != "cuda" or values.dtype != torch.uint8:
+            raise ValueError(f"{name} values must be a uint8 CUDA tensor")
+        if values.ndim != 2 or not values.is_contiguous():
+            raise ValueError(f"{name} values must be a contiguous matrix")
+    rows, half = values.shape
+    cols = 2 * half
+    if not (1 <= rows <= _MAX_EXTENT and 1 <= cols <= _MAX_EXTENT):
+        raise ValueError(f"{name} extents must be positive and at most {_MAX_EXTENT}")
+    if cols % MXFP8_TILE_SIZE:
         raise ValueError(f"{name} must have a multiple of {MXFP8_TILE_SIZE} columns")
-    if scales.dtype != torch.uint8 or scales.shape != (-(-rows // 128), cols // 128, 32, 16):
+    if scales.dtype is not torch.uint8 or scales.shape != (-(-rows // 128), cols // 128, 32, 16):
         raise ValueError(f"{name} scales must be uint8 [{-(-rows // 128)}, {cols // 128}, 32, 16]")
-    if not scales.is_contiguous() or scales.device != values.device:
+    if not scales.is_contiguous() or not _same_device(scales, values):
         raise ValueError(f"{name} scales must be contiguous and on the values' device")
-    if device is not None and values.device != device:
+    if x is not None and not _same_device(values, x):
         raise ValueError(f"{name} must be on x's device")
     return rows, cols
 
@@ -397,34 +423,27 @@ def quantize_mxfp4(weight: torch.Tensor) -> Mxfp4Tensor:
     a NaN or an infinity stands for NaN.
     """
 
-    _check_bf16_matrix("weight", weight)
-    _check_extents(weight)
+    _need_bf16_matrix("weight", weight)
     rows, cols = weight.shape
     if cols % MXFP8_TILE_SIZE:
         raise ValueError(f"weight must have a multiple of {MXFP8_TILE_SIZE} columns")
     values = torch.empty(rows, cols // 2, dtype=torch.uint8, device=weight.device)
     scales = torch.empty(-(-rows // 128), cols // 128, 32, 16, dtype=torch.uint8, device=weight.device)
-    with torch.cuda.device(weight.device):
-        _lib.check(
-            _lib.library().ce4b_quantize_mxfp4(
-                weight.data_ptr(), values.data_ptr(), scales.data_ptr(), rows, cols, _stream(weight)
-            )
-        )
+    _call(
+        "ce4b_quantize_mxfp4", weight, weight.data_ptr(), values.data_ptr(), scales.data_ptr(), rows, cols,
+    )
     return Mxfp4Tensor(values=values, scales=scales)
 
 
 def dequantize_mxfp4(weight: Mxfp4Tensor) -> torch.Tensor:
     """The BF16 matrix that an MXFP4 weight stands for (exact)."""
 
-    rows, cols = _check_mxfp4("weight", weight)
+    rows, cols = _need_mxfp4("weight", weight)
     values = weight.values
     out = torch.empty(rows, cols, dtype=torch.bfloat16, device=values.device)
-    with torch.cuda.device(values.device):
-        _lib.check(
-            _lib.library().ce4b_dequantize_mxfp4(
-                values.data_ptr(), weight.scales.data_ptr(), out.data_ptr(), rows, cols, _stream(values)
-            )
-        )
+    _call(
+        "ce4b_dequantize_mxfp4", values, values.data_ptr(), weight.scales.data_ptr(), out.data_ptr(), rows, cols,
+    )
     return out
 
 
@@ -436,25 +455,19 @@ def mxfp4_linear(
     more rows read the weight again for every 64. A NaN or an infinity in a row of ``x``
     makes that row of the result non-finite."""
 
-    _check_bf16_matrix("x", x)
-    _check_extents(x)
-    n, k = _check_mxfp4("weight", weight, x.device)
+    _need_bf16_matrix("x", x)
+    n, k = _need_mxfp4("weight", weight, x)
     rows = x.shape[0]
     if x.shape[1] != k:
         raise ValueError("MXFP4 product reduction dimensions do not match")
     if residual is not None:
-        _check_bf16_matrix("residual", residual)
-        if tuple(residual.shape) != (rows, n) or residual.device != x.device:
+        _need_bf16_matrix("residual", residual)
+        if residual.shape != (rows, n) or not _same_device(residual, x):
             raise ValueError(f"residual must have shape [{rows}, {n}] on x's device")
-    out = torch.empty(rows, n, dtype=torch.bfloat16, device=x.device)
-    with torch.cuda.device(x.device):
-        _lib.check(
-            _lib.library().ce4b_mxfp4_linear(
-                x.data_ptr(), weight.values.data_ptr(), weight.scales.data_ptr(),
-                None if residual is None else residual.data_ptr(), out.data_ptr(), rows, n, k,
-                _stream(x),
-            )
-        )
+    out = x.new_empty(rows, n)
+    _call(
+        "ce4b_mxfp4_linear", x, x.data_ptr(), weight.values.data_ptr(), weight.scales.data_ptr(), None if residual is None else residual.data_ptr(), out.data_ptr(), rows, n, k,
+    )
     return out
 
 
@@ -463,22 +476,17 @@ def mxfp4_swiglu(x: torch.Tensor, gate_up_weight: Mxfp4Tensor) -> torch.Tensor:
     (gate rows first): the first product of a dense block for a few BF16 rows, FP32 until
     the one rounding at the end. Rows as in :func:`mxfp4_linear`."""
 
-    _check_bf16_matrix("x", x)
-    _check_extents(x)
-    wide, k = _check_mxfp4("gate_up_weight", gate_up_weight, x.device)
+    _need_bf16_matrix("x", x)
+    wide, k = _need_mxfp4("gate_up_weight", gate_up_weight, x)
     rows = x.shape[0]
     if x.shape[1] != k:
         raise ValueError("MXFP4 product reduction dimensions do not match")
     if wide % 2:
         raise ValueError("gate_up_weight must have an even number of rows")
-    hidden = torch.empty(rows, wide // 2, dtype=torch.bfloat16, device=x.device)
-    with torch.cuda.device(x.device):
-        _lib.check(
-            _lib.library().ce4b_mxfp4_swiglu(
-                x.data_ptr(), gate_up_weight.values.data_ptr(), gate_up_weight.scales.data_ptr(),
-                hidden.data_ptr(), rows, wide // 2, k, _stream(x),
-            )
-        )
+    hidden = x.new_empty(rows, wide // 2)
+    _call(
+        "ce4b_mxfp4_swiglu", x, x.data_ptr(), gate_up_weight.values.data_ptr(), gate_up_weight.scales.data_ptr(), hidden.data_ptr(), rows, wide // 2, k,
+    )
     return hidden
 
 

@@ -40,12 +40,12 @@ __device__ __forceinline__ uint4 load_stream(const uint8_t* p) {
   return v;
 }
 
-template <int NT, bool SWIGLU>
+template <int NT, int MT, bool SWIGLU>
 __global__ void __launch_bounds__(32 * kWarps)
     mx4_vector_kernel(const bf16* x, const uint8_t* codes, const uint8_t* scales,
                       const bf16* residual, bf16* out, int rows, int n, int k) {
-  constexpr int kCols = SWIGLU ? 8 : 16;  // output columns per CTA
-  __shared__ float part[kWarps][8 * NT][17];
+  constexpr int kCols = (SWIGLU ? 8 : 16) * MT;  // output columns per CTA
+  __shared__ float part[kWarps][8 * NT][16 * MT + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int col0 = blockIdx.x * kCols, row0 = blockIdx.y * 8 * NT;
@@ -53,15 +53,18 @@ __global__ void __launch_bounds__(32 * kWarps)
   grid_dependency_wait();
   grid_launch_dependents();
 
-  const uint8_t* code_ptr[2];
-  const uint8_t* scale_ptr[2];
+  // Fragment row h of tile m: weight rows past the last one read it again, unused.
+  const uint8_t* code_ptr[MT][2];
+  const uint8_t* scale_ptr[MT][2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    // Rows past the last one read it again; their sums are not used.
-    const int wrow = SWIGLU ? min(col0 + g, n - 1) + h * n : min(col0 + g + 8 * h, n - 1);
-    code_ptr[h] = codes + static_cast<size_t>(wrow) * (k / 2) + t * 16;
-    scale_ptr[h] = scales + static_cast<size_t>(wrow / 128) * kblocks * 512 + (wrow % 32) * 16 +
-                   (wrow / 32 % 4) * 4 + t;
+  for (int m = 0; m < MT; ++m) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int wrow = SWIGLU ? min(col0 + 8 * m + g, n - 1) + h * n : min(col0 + 16 * m + 8 * h + g, n - 1);
+      code_ptr[m][h] = codes + static_cast<size_t>(wrow) * (k / 2) + t * 16;
+      scale_ptr[m][h] = scales + static_cast<size_t>(wrow / 128) * kblocks * 512 + (wrow % 32) * 16 +
+                        (wrow / 32 % 4) * 4 + t;
+    }
   }
   const bf16* x_ptr[NT];
 #pragma unroll
@@ -69,17 +72,21 @@ __global__ void __launch_bounds__(32 * kWarps)
     x_ptr[j] = row0 + 8 * j + g < rows ? x + static_cast<size_t>(row0 + 8 * j + g) * k + t * 32 : nullptr;
   }
 
-  float acc[NT][4] = {};
-  uint4 q[2];
-  uint32_t sc[2];
-  int kb = warp;
-  if (kb < kblocks) {
+  float acc[MT][NT][4] = {};
+  uint4 q[MT][2];
+  uint32_t sc[MT][2];
+  auto load = [&](int kb) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      q[h] = load_stream(code_ptr[h] + kb * 64);
-      sc[h] = scale_ptr[h][static_cast<size_t>(kb) * 512];
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        q[m][h] = load_stream(code_ptr[m][h] + kb * 64);
+        sc[m][h] = scale_ptr[m][h][static_cast<size_t>(kb) * 512];
+      }
     }
-  }
+  };
+  int kb = warp;
+  if (kb < kblocks) load(kb);
   while (kb < kblocks) {
     uint4 xv[NT][4];
 #pragma unroll
@@ -90,52 +97,64 @@ __global__ void __launch_bounds__(32 * kWarps)
                                        : make_uint4(0u, 0u, 0u, 0u);
       }
     }
-    const uint4 c[2] = {q[0], q[1]};
-    const uint32_t s[2] = {sc[0], sc[1]};
-    kb += kWarps;
-    if (kb < kblocks) {
+    uint4 c[MT][2];
+    uint32_t s[MT][2], f[MT][2], top = 0;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        q[h] = load_stream(code_ptr[h] + kb * 64);
-        sc[h] = scale_ptr[h][static_cast<size_t>(kb) * 512];
+        c[m][h] = q[m][h];
+        s[m][h] = sc[m][h];
+        f[m][h] = mx4_factor(s[m][h]);
+        top = max(top, s[m][h]);
       }
     }
-    const uint32_t f[2] = {mx4_factor(s[0]), mx4_factor(s[1])};
-    const bool wide = __any_sync(0xffffffffu, max(s[0], s[1]) > 128u);
+    kb += kWarps;
+    if (kb < kblocks) load(kb);
+    const bool wide = __any_sync(0xffffffffu, top > 128u);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      uint32_t a[2][4];
+      uint4 b[NT];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        mx4_expand(i == 0 ? c[h].x : i == 1 ? c[h].y : i == 2 ? c[h].z : c[h].w, f[h], a[h]);
-        if (wide) {
+      for (int j = 0; j < NT; ++j) b[j] = permute_x(xv[j][i]);
 #pragma unroll
-          for (int m = 0; m < 4; ++m) a[h][m] = mul_bf16x2(a[h][m], mx4_factor2(s[h]));
+      for (int m = 0; m < MT; ++m) {
+        uint32_t a[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          mx4_expand(i == 0 ? c[m][h].x : i == 1 ? c[m][h].y : i == 2 ? c[m][h].z : c[m][h].w, f[m][h], a[h]);
+          if (wide) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[h][e] = mul_bf16x2(a[h][e], mx4_factor2(s[m][h]));
+          }
         }
-      }
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const uint4 b = permute_x(xv[j][i]);
-        mma_bf16(acc[j], a[0][0], a[1][0], a[0][1], a[1][1], b.x, b.y);
-        mma_bf16(acc[j], a[0][2], a[1][2], a[0][3], a[1][3], b.z, b.w);
+        for (int j = 0; j < NT; ++j) {
+          mma_bf16(acc[m][j], a[0][0], a[1][0], a[0][1], a[1][1], b[j].x, b[j].y);
+          mma_bf16(acc[m][j], a[0][2], a[1][2], a[0][3], a[1][3], b[j].z, b[j].w);
+        }
       }
     }
   }
   // A lane holds weight rows g and g + 8, activation rows 2t and 2t + 1 of each 8.
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
+  for (int m = 0; m < MT; ++m) {
 #pragma unroll
-    for (int m = 0; m < 4; ++m) part[warp][8 * j + 2 * t + (m & 1)][g + 8 * (m >> 1)] = acc[j][m];
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[warp][8 * j + 2 * t + (e & 1)][16 * m + g + 8 * (e >> 1)] = acc[m][j][e];
+    }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < 8 * NT * kCols; i += 32 * kWarps) {
     const int r = i / kCols, c = i % kCols;
     if (row0 + r >= rows || col0 + c >= n) continue;
+    const int at_part = SWIGLU ? c / 8 * 16 + c % 8 : c;
     float y = 0.0f, u = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      y += part[w][r][c];
-      if (SWIGLU) u += part[w][r][8 + c];
+      y += part[w][r][at_part];
+      if (SWIGLU) u += part[w][r][at_part + 8];
     }
     if (SWIGLU) y = y / (1.0f + expf(-y)) * u;
     const size_t at = static_cast<size_t>(row0 + r) * n + col0 + c;
@@ -144,23 +163,26 @@ __global__ void __launch_bounds__(32 * kWarps)
   }
 }
 
-template <int NT, bool SWIGLU>
+template <int NT, int MT, bool SWIGLU>
 void launch_vector(const bf16* x, const uint8_t* codes, const uint8_t* scales, const bf16* residual,
                    bf16* out, int rows, int n, int k, cudaStream_t s) {
-  constexpr int kCols = SWIGLU ? 8 : 16;
+  constexpr int kCols = (SWIGLU ? 8 : 16) * MT;
   const dim3 grid(static_cast<unsigned>((n + kCols - 1) / kCols), static_cast<unsigned>((rows + 8 * NT - 1) / (8 * NT)));
-  launch(mx4_vector_kernel<NT, SWIGLU>, grid, 32 * kWarps, 0, 0, s, x, codes, scales, residual, out, rows, n, k);
+  launch(mx4_vector_kernel<NT, MT, SWIGLU>, grid, 32 * kWarps, 0, 0, s, x, codes, scales, residual, out, rows, n, k);
 }
 
+#ifndef VMT
+#define VMT 1
+#endif
 template <bool SWIGLU>
 void product(const bf16* x, const uint8_t* codes, const uint8_t* scales, const bf16* residual,
              bf16* out, int rows, int n, int k, cudaStream_t s) {
   if (rows <= 8) {
-    launch_vector<1, SWIGLU>(x, codes, scales, residual, out, rows, n, k, s);
+    launch_vector<1, VMT, SWIGLU>(x, codes, scales, residual, out, rows, n, k, s);
   } else if (rows <= 16) {
-    launch_vector<2, SWIGLU>(x, codes, scales, residual, out, rows, n, k, s);
+    launch_vector<2, VMT, SWIGLU>(x, codes, scales, residual, out, rows, n, k, s);
   } else if (rows <= 32) {
-    launch_vector<4, SWIGLU>(x, codes, scales, residual, out, rows, n, k, s);
+    launch_vector<4, VMT, SWIGLU>(x, codes, scales, residual, out, rows, n, k, s);
   } else {
     mx4_product_tc(x, codes, scales, residual, out, rows, n, k, SWIGLU, s);
   }

@@ -27,6 +27,13 @@ __device__ __forceinline__ float mx_scale_inverse(uint8_t code) {
   return biased >= 1u ? __uint_as_float(biased << 23) : __uint_as_float(0x00400000u);
 }
 
+// Four values times `inv` as packed E4M3 codes.
+__device__ __forceinline__ uint32_t mx_codes4(float a, float b, float c, float d, float inv) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c * inv, d * inv), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+
 // Quantise 32 values (one scale block) to packed E4M3 codes; returns the scale code.
 __device__ __forceinline__ uint8_t mx_quantize32(const float (&v)[32], uint32_t (&codes)[8]) {
   float amax = 0.0f;
@@ -35,13 +42,7 @@ __device__ __forceinline__ uint8_t mx_quantize32(const float (&v)[32], uint32_t 
   const uint8_t sc = mx_scale_code(amax);
   const float inv = mx_scale_inverse(sc);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * j] * inv, v[4 * j + 1] * inv),
-                                                 __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(
-        make_float2(v[4 * j + 2] * inv, v[4 * j + 3] * inv), __NV_SATFINITE, __NV_E4M3);
-    codes[j] = lo | (hi << 16);
-  }
+  for (int j = 0; j < 8; ++j) codes[j] = mx_codes4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3], inv);
   return sc;
 }
 

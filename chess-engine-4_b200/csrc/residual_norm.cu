@@ -1,7 +1,10 @@
 // Residual addition and RMSNorm of rows (kernel-op API add_rmsnorm_forward and
 // add_rmsnorm_mxfp8): s = bf16(x + residual), n = bf16(s * (mean(s^2) + eps)^(-1/2) * w), n as
 // BF16 or as the MXFP8 codes and scales of that BF16 value.
+#include <algorithm>
+
 #include "internal.h"
+#include "launch.cuh"
 #include "mxfp8.cuh"
 #include "ptx.cuh"
 
@@ -28,30 +31,187 @@ __device__ __forceinline__ RowScale row_scale(double sum, double inv_width, floa
 
 // s * (hi + lo) * w: q is the FP32 rounding of the product and e the rest, so that q + e is the
 // product rounded to FP32 once (about 2^-46 of it is lost before). An overflowing q has no rest.
-__device__ __forceinline__ float scale_round(float s, float w, const RowScale& f) {
+__device__ __forceinline__ float scale_product(float s, float w, const RowScale& f) {
   const float t = s * f.hi;
   const float te = fmaf(s, f.lo, fmaf(s, f.hi, -t));
   const float q = t * w;
   const float e = fmaf(te, w, fmaf(t, w, -q));
-  return bf16_round(fabsf(q) <= 3.0e38f ? q + e : q);
+  return fabsf(q) <= 3.0e38f ? q + e : q;
 }
 
-__device__ __forceinline__ double block_sum(double v) {
-  __shared__ double part[32];
+__device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  const int warps = blockDim.x / 32;
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x / 32] = v;
-  __syncthreads();
-  v = 0.0;
-  for (int i = 0; i < warps; ++i) v += part[i];
   return v;
 }
 
-// One block per row (rows in blockIdx.x); the row is read again for the second pass.
-__global__ void add_rmsnorm_kernel(const bf16* x, const bf16* residual, const bf16* w, bf16* sum,
-                                   bf16* out, uint8_t* codes, uint8_t* scales, int rows, int width,
-                                   double inv_width, float eps) {
+// Eight BF16 values of a row: a 16-byte access where the whole chunk belongs to the row, single
+// elements at the ends of rows that do not start or end on 16 bytes. `from`..`to` are the
+// chunk's elements that the row owns.
+__device__ __forceinline__ uint4 load_chunk(const bf16* p, int from, int to) {
+  if (from == 0 && to == 8) return *reinterpret_cast<const uint4*>(p);
+  uint32_t v[4] = {};
+  const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (j >= from && j < to) v[j / 2] |= static_cast<uint32_t>(u[j]) << (16 * (j % 2));
+  }
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+__device__ __forceinline__ void store_chunk(bf16* p, const uint32_t (&v)[4], int from, int to) {
+  if (from == 0 && to == 8) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(v[0], v[1], v[2], v[3]);
+    return;
+  }
+  uint16_t* u = reinterpret_cast<uint16_t*>(p);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (j >= from && j < to) u[j] = static_cast<uint16_t>(v[j / 2] >> (16 * (j % 2)));
+  }
+}
+
+// A row is held in the registers of TPR threads, V chunks of eight columns each, and read and
+// written once. ALIGNED: rows start and end on 16 bytes (width % 8 == 0), and a thread keeps
+// its part of w over the rows it takes. Otherwise chunks are the aligned 16 bytes of the
+// matrix, and the row's first and last one are accessed by elements.
+template <int V, int TPR, bool ALIGNED, bool MX>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
+    add_rmsnorm_kernel(const bf16* x, const bf16* residual, const bf16* __restrict__ w, bf16* sum,
+                       bf16* out, uint8_t* codes, uint8_t* scales, int rows, int width,
+                       double inv_width, float eps) {
+  constexpr int kThreads = TPR > 256 ? TPR : 256;
+  constexpr int kRows = kThreads / TPR;  // rows of a block at a time
+  constexpr int kWarps = TPR / 32;       // warps of a row
+  __shared__ double part[2][kThreads / 32];
+  const int lane = threadIdx.x % TPR;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  uint4 wv[V];
+  if constexpr (ALIGNED) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = (i * TPR + lane) * 8;
+      wv[i] = c < width ? *reinterpret_cast<const uint4*>(w + c) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  const int last = MX ? (rows + 127) / 128 * 128 : rows;
+  int turn = 0;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * kRows; r0 < last;
+       r0 += static_cast<int64_t>(gridDim.x) * kRows, turn ^= 1) {
+    const int64_t row = r0 + threadIdx.x / TPR;
+    const bool live = row < rows;
+    // The row's chunks start at element `begin` of the matrix; column 0 is `shift` after it.
+    const int64_t first = row * width;
+    const int shift = ALIGNED ? 0 : static_cast<int>(first & 7);
+    const int64_t begin = first - shift;
+    uint4 v[V], r[V];
+    auto bounds = [&](int i, int& from, int& to) {
+      const int c = (i * TPR + lane) * 8;  // of the chunks' elements
+      from = ALIGNED ? 0 : max(shift - c, 0);
+      to = ALIGNED ? 8 : min(shift + width - c, 8);
+      return live && (ALIGNED ? c < width : c < shift + width);
+    };
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      int from, to;
+      const bool own = bounds(i, from, to);
+      const int64_t at = begin + (i * TPR + lane) * 8;
+      v[i] = r[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (own) v[i] = load_chunk(x + at, from, to);
+      if (own && residual != nullptr) r[i] = load_chunk(residual + at, from, to);
+    }
+    double ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      uint32_t* q = reinterpret_cast<uint32_t*>(&v[i]);
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(&r[i]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float2 s = unpack_bf16x2(q[j]);
+        if (residual != nullptr) {
+          const float2 t = unpack_bf16x2(p[j]);
+          q[j] = pack_bf16x2(s.x + t.x, s.y + t.y);
+          s = unpack_bf16x2(q[j]);
+        }
+        const double a = s.x, b = s.y;
+        ss = fma(a, a, ss);
+        ss = fma(b, b, ss);
+      }
+      int from, to;
+      if (residual != nullptr && bounds(i, from, to)) {
+        const uint32_t words[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        store_chunk(sum + begin + (i * TPR + lane) * 8, words, from, to);
+      }
+    }
+    ss = warp_sum(ss);
+    if constexpr (kWarps > 1) {
+      const int warp = threadIdx.x / 32;
+      if (threadIdx.x % 32 == 0) part[turn][warp] = ss;
+      __syncthreads();
+      ss = 0.0;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) ss += part[turn][warp / kWarps * kWarps + i];
+    }
+    const RowScale f = row_scale(ss, inv_width, eps);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      int from, to;
+      const bool own = bounds(i, from, to);
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(&v[i]);
+      const int c = (i * TPR + lane) * 8;
+      float n[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 s = unpack_bf16x2(q[j]);
+        float2 u;
+        if constexpr (ALIGNED) {
+          u = unpack_bf16x2(reinterpret_cast<const uint32_t*>(&wv[i])[j]);
+        } else {
+          const int col = c - shift + 2 * j;
+          u.x = own && 2 * j >= from && 2 * j < to ? __bfloat162float(w[col]) : 0.0f;
+          u.y = own && 2 * j + 1 >= from && 2 * j + 1 < to ? __bfloat162float(w[col + 1]) : 0.0f;
+        }
+        n[2 * j] = scale_product(s.x, u.x, f);
+        n[2 * j + 1] = scale_product(s.y, u.y, f);
+      }
+      uint32_t words[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) words[j] = pack_bf16x2(n[2 * j], n[2 * j + 1]);
+      if constexpr (!MX) {
+        if (own) store_chunk(out + begin + c, words, from, to);
+      } else {
+        // Four neighbouring threads hold the 32 columns of a scale block.
+        float m[8], amax = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 t = unpack_bf16x2(words[j]);
+          m[2 * j] = t.x, m[2 * j + 1] = t.y;
+          amax = fmaxf(amax, fmaxf(fabsf(t.x), fabsf(t.y)));
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const uint8_t sc = mx_scale_code(amax);
+        const float inv = mx_scale_inverse(sc);
+        uint2 e;
+        e.x = mx_codes4(m[0], m[1], m[2], m[3], inv);
+        e.y = mx_codes4(m[4], m[5], m[6], m[7], inv);
+        if (own) *reinterpret_cast<uint2*>(codes + first + c) = e;
+        if (row < last && c < width && lane % 4 == 0) {
+          scales[mx_scale_offset(static_cast<int>(row), c / 32, width / 128)] = live ? sc : 0;
+        }
+      }
+    }
+  }
+}
+
+// Any width, alignment and form, one block per row (rows in blockIdx.x): rows too wide for the
+// registers above, and matrices whose buffers start off 16 bytes. The row's sum is read again
+// (from the cache) for the second pass.
+__global__ void add_rmsnorm_any_kernel(const bf16* x, const bf16* residual, const bf16* w, bf16* sum,
+                                       bf16* out, uint8_t* codes, uint8_t* scales, int rows,
+                                       int width, double inv_width, float eps) {
+  __shared__ double part[32];
   const int row = blockIdx.x;
   if (row >= rows) {  // padding rows of the last scale tile
     for (int b = threadIdx.x; b < width / 32; b += blockDim.x) scales[mx_scale_offset(row, b, width / 128)] = 0;
@@ -67,21 +227,24 @@ __global__ void add_rmsnorm_kernel(const bf16* x, const bf16* residual, const bf
     }
     ss = fma(static_cast<double>(s), static_cast<double>(s), ss);
   }
-  ss = block_sum(ss);
+  ss = warp_sum(ss);
+  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = ss;
+  __syncthreads();  // also before the sum of other threads' columns is read below
+  ss = 0.0;
+  for (int i = 0; i < static_cast<int>(blockDim.x) / 32; ++i) ss += part[i];
   const RowScale f = row_scale(ss, inv_width, eps);
   const bf16* src = residual != nullptr ? sum : x;
   if (codes == nullptr) {
     for (int c = threadIdx.x; c < width; c += blockDim.x) {
       out[at + c] = __float2bfloat16_rn(
-          scale_round(__bfloat162float(src[at + c]), __bfloat162float(w[c]), f));
+          scale_product(__bfloat162float(src[at + c]), __bfloat162float(w[c]), f));
     }
     return;
   }
-  __syncthreads();  // the sum of other threads' columns is read below
   for (int b = threadIdx.x; b < width / 32; b += blockDim.x) {
     float v[32];
     for (int j = 0; j < 32; ++j) {
-      v[j] = scale_round(__bfloat162float(src[at + b * 32 + j]), __bfloat162float(w[b * 32 + j]), f);
+      v[j] = bf16_round(scale_product(__bfloat162float(src[at + b * 32 + j]), __bfloat162float(w[b * 32 + j]), f));
     }
     uint32_t q[8];
     const uint8_t sc = mx_quantize32(v, q);
@@ -91,14 +254,68 @@ __global__ void add_rmsnorm_kernel(const bf16* x, const bf16* residual, const bf
   }
 }
 
+struct NormArgs {
+  const bf16 *x, *residual, *w;
+  bf16 *sum, *out;
+  uint8_t *codes, *scales;
+  int rows, width;
+  float eps;
+  cudaStream_t s;
+};
+
+template <int V, int TPR, bool ALIGNED, bool MX>
+void launch_norm(const NormArgs& a) {
+  constexpr int kThreads = TPR > 256 ? TPR : 256;
+  constexpr int kRows = kThreads / TPR;
+  const int64_t rows = MX ? (static_cast<int64_t>(a.rows) + 127) / 128 * 128 : a.rows;
+  // Blocks that stay on the GPU (2048 threads an SM at most) and take rows in turn.
+  const int64_t grid = std::min<int64_t>((rows + kRows - 1) / kRows, static_cast<int64_t>(sm_count()) * (2048 / kThreads));
+  launch(add_rmsnorm_kernel<V, TPR, ALIGNED, MX>, dim3(static_cast<unsigned>(grid)), kThreads, 0, 0, a.s,
+         a.x, a.residual, a.w, a.sum, a.out, a.codes, a.scales, a.rows, a.width, 1.0 / a.width, a.eps);
+}
+
+template <bool ALIGNED, bool MX>
+bool launch_rows(const NormArgs& a) {
+  const int chunks = ALIGNED ? a.width / 8 : (a.width + 14) / 8;
+  // Few rows: as many threads per row as it has chunks, for the shortest chain. Many rows: four
+  // chunks a thread, so that a row is a warp's or few warps' business and its sum needs few
+  // steps across warps.
+  const bool few = static_cast<int64_t>(a.rows) * chunks <= static_cast<int64_t>(sm_count()) * 2048;
+  if (few && chunks <= 1024) {
+    if (chunks <= 32) return launch_norm<1, 32, ALIGNED, MX>(a), true;
+    if (chunks <= 64) return launch_norm<1, 64, ALIGNED, MX>(a), true;
+    if (chunks <= 128) return launch_norm<1, 128, ALIGNED, MX>(a), true;
+    if (chunks <= 256) return launch_norm<1, 256, ALIGNED, MX>(a), true;
+    if (chunks <= 512) return launch_norm<1, 512, ALIGNED, MX>(a), true;
+    return launch_norm<1, 1024, ALIGNED, MX>(a), true;
+  }
+  if (chunks <= 32) return launch_norm<1, 32, ALIGNED, MX>(a), true;
+  if (chunks <= 64) return launch_norm<2, 32, ALIGNED, MX>(a), true;
+  if (chunks <= 128) return launch_norm<4, 32, ALIGNED, MX>(a), true;
+  if (chunks <= 256) return launch_norm<4, 64, ALIGNED, MX>(a), true;
+  if (chunks <= 512) return launch_norm<4, 128, ALIGNED, MX>(a), true;
+  if (chunks <= 1024) return launch_norm<4, 256, ALIGNED, MX>(a), true;
+  if (chunks <= 2048) return launch_norm<4, 512, ALIGNED, MX>(a), true;
+  return false;
+}
+
 }  // namespace
 
 void add_rmsnorm_rows(const bf16* x, const bf16* residual, const bf16* w, bf16* sum, bf16* out,
                       uint8_t* codes, uint8_t* scales, int rows, int width, float eps,
                       cudaStream_t s) {
-  const int grid = codes != nullptr ? (rows + 127) / 128 * 128 : rows;
-  add_rmsnorm_kernel<<<grid, 256, 0, s>>>(x, residual, w, sum, out, codes, scales, rows, width,
-                                          1.0 / width, eps);
+  const NormArgs a{x, residual, w, sum, out, codes, scales, rows, width, eps, s};
+  auto wide = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+  const bool mx = codes != nullptr;
+  if (wide(x) && wide(residual) && (residual == nullptr || wide(sum)) && (mx || wide(out))) {
+    const bool aligned = width % 8 == 0 && wide(w);
+    if (mx ? aligned && launch_rows<true, true>(a) : aligned ? launch_rows<true, false>(a) : launch_rows<false, false>(a)) {
+      return;
+    }
+  }
+  const int grid = mx ? (rows + 127) / 128 * 128 : rows;
+  add_rmsnorm_any_kernel<<<grid, 256, 0, s>>>(x, residual, w, sum, out, codes, scales, rows, width,
+                                              1.0 / width, eps);
   check_cuda(cudaGetLastError(), "add_rmsnorm launch");
 }
 
