@@ -632,7 +632,8 @@ int ce4b_quantize_mxfp4(const void* x_dev, void* codes_dev, void* scales_dev, in
     require(x_dev && codes_dev && scales_dev, "null pointer");
     require(rows >= 1 && cols >= 1, "extents must be positive");
     require(cols % 128 == 0, "MXFP4 columns must be a multiple of 128");
-    require(aligned(x_dev, 16) && aligned(codes_dev, 16), "MXFP4 buffers must be 16-byte aligned");
+    require(aligned(x_dev, 16) && aligned(codes_dev, 16) && aligned(scales_dev, 16),
+            "MXFP4 buffers must be 16-byte aligned");
     mx4_quantize(static_cast<const bf16*>(x_dev), static_cast<uint8_t*>(codes_dev),
                  static_cast<uint8_t*>(scales_dev), rows, cols, as_stream(stream));
   });
@@ -644,7 +645,8 @@ int ce4b_dequantize_mxfp4(const void* codes_dev, const void* scales_dev, void* o
     require(codes_dev && scales_dev && out_dev, "null pointer");
     require(rows >= 1 && cols >= 1, "extents must be positive");
     require(cols % 128 == 0, "MXFP4 columns must be a multiple of 128");
-    require(aligned(codes_dev, 16) && aligned(out_dev, 16), "MXFP4 buffers must be 16-byte aligned");
+    require(aligned(codes_dev, 16) && aligned(scales_dev, 16) && aligned(out_dev, 16),
+            "MXFP4 buffers must be 16-byte aligned");
     mx4_dequantize(static_cast<const uint8_t*>(codes_dev), static_cast<const uint8_t*>(scales_dev),
                    static_cast<bf16*>(out_dev), rows, cols, as_stream(stream));
   });

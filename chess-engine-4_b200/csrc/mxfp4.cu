@@ -6,6 +6,8 @@
 #include <algorithm>
 
 #include "internal.h"
+#include "launch.cuh"
+#include "mxfp4.cuh"
 #include "mxfp8.cuh"
 #include "ptx.cuh"
 
@@ -24,81 +26,99 @@ __device__ __forceinline__ uint32_t mx4_scale_code(uint32_t amax_bits) {  // of 
   return code < 88u + 2u ? 88u : code - 2u;
 }
 
-__device__ __forceinline__ float mx4_value(uint32_t nibble) {
-  const uint32_t m = nibble & 7u;
-  const float v = m < 4u ? 0.5f * m : (m == 4u ? 2.0f : (m == 5u ? 3.0f : (m == 6u ? 4.0f : 6.0f)));
-  return nibble & 8u ? -v : v;
-}
+// Both kernels take [16 rows][128 columns] tiles with 256 threads, eight columns a thread (16
+// bytes of BF16, 4 bytes of codes), and kTiles column tiles at once for loads in flight. Sixteen
+// threads hold the four scale bytes of a row in a tile, one 32-bit word.
+constexpr int kTiles = 4;
 
-__device__ __forceinline__ float mx4_scale(uint32_t code) {  // 2^(code - 127); NaN for 255
-  if (code == 255u) return __uint_as_float(0x7FFFFFFFu);
-  return code == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(code << 23);
-}
-
-// One thread per (row, 32-column group); rows past the last one zero their scale bytes.
-__global__ void mx4_quantize_kernel(const bf16* __restrict__ x, uint8_t* __restrict__ codes,
-                                    uint8_t* __restrict__ scales, int rows, int cols) {
-  const int groups = cols / 32;
-  const int64_t total = static_cast<int64_t>((rows + 127) / 128 * 128) * groups;
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int row = static_cast<int>(i / groups);
-    const int g = static_cast<int>(i - static_cast<int64_t>(row) * groups);
-    uint32_t code = 0;
-    if (row < rows) {
-      const bf16* src = x + static_cast<size_t>(row) * cols + g * 32;
-      uint32_t amax = 0;
-      for (int j = 0; j < 32; ++j) {
-        amax = max(amax, __float_as_uint(__bfloat162float(src[j])) & 0x7FFFFFFFu);
-      }
-      code = mx4_scale_code(amax);
-      const float inv = code == 255u ? 0.0f : mx_scale_inverse(static_cast<uint8_t>(code));
-      uint8_t* dst = codes + static_cast<size_t>(row) * (cols / 2) + g * 16;
-      for (int j = 0; j < 16; ++j) {
-        const float2 v = make_float2(__bfloat162float(src[2 * j]) * inv, __bfloat162float(src[2 * j + 1]) * inv);
-        dst[j] = code == 255u ? 0 : __nv_cvt_float2_to_fp4x2(v, __NV_E2M1, cudaRoundNearest);
+__global__ void __launch_bounds__(256)
+    mx4_quantize_kernel(const bf16* __restrict__ x, uint8_t* __restrict__ codes,
+                        uint8_t* __restrict__ scales, int rows, int cols) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16;
+  const int lane = threadIdx.x % 16;
+  const int col_tiles = cols / 128;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  uint32_t* const scale_row = reinterpret_cast<uint32_t*>(scales) +
+                              (row / 128 * col_tiles) * 128 + (row % 32) * 4 + row / 32 % 4;
+  for (int t0 = blockIdx.y * kTiles; t0 < col_tiles; t0 += gridDim.y * kTiles) {
+    uint4 v[kTiles];
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) {
+      v[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < rows && t0 + j < col_tiles) {
+        v[j] = *reinterpret_cast<const uint4*>(x + row * cols + (t0 + j) * 128 + lane * 8);
       }
     }
-    scales[mx_scale_offset(row, g, cols / 128)] = static_cast<uint8_t>(code);
-  }
-}
-
-__global__ void mx4_dequantize_kernel(const uint8_t* __restrict__ codes,
-                                      const uint8_t* __restrict__ scales, bf16* __restrict__ out,
-                                      int rows, int cols) {
-  const int groups = cols / 32;
-  const int64_t total = static_cast<int64_t>(rows) * groups;
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int row = static_cast<int>(i / groups);
-    const int g = static_cast<int>(i - static_cast<int64_t>(row) * groups);
-    const float s = mx4_scale(scales[mx_scale_offset(row, g, cols / 128)]);
-    const uint8_t* src = codes + static_cast<size_t>(row) * (cols / 2) + g * 16;
-    bf16* dst = out + static_cast<size_t>(row) * cols + g * 32;
-    for (int j = 0; j < 16; ++j) {
-      dst[2 * j] = __float2bfloat16_rn(mx4_value(src[j] & 15u) * s);
-      dst[2 * j + 1] = __float2bfloat16_rn(mx4_value(src[j] >> 4) * s);
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) {
+      const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+      // Magnitudes of BF16 numbers compare like their bits, infinities and NaN on top.
+      uint32_t top = __vmaxu2(__vmaxu2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu),
+                              __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
+      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t code = mx4_scale_code(max(top << 16, top & 0xFFFF0000u));
+      const float inv = mx_scale_inverse(static_cast<uint8_t>(code));
+      uint32_t q = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack_bf16x2(w[i]);
+        q |= static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(make_float2(f.x * inv, f.y * inv), __NV_E2M1, cudaRoundNearest)) << (8 * i);
+      }
+      if (code == 255u) q = 0;
+      uint32_t word = row < rows ? code << (8 * (lane / 4)) : 0u;  // padding rows: 0
+      word |= __shfl_xor_sync(0xffffffffu, word, 4);
+      word |= __shfl_xor_sync(0xffffffffu, word, 8);
+      if (t0 + j < col_tiles) {
+        if (row < rows) *reinterpret_cast<uint32_t*>(codes + row * (cols / 2) + (t0 + j) * 64 + lane * 4) = q;
+        if (lane == 0) scale_row[static_cast<int64_t>(t0 + j) * 128] = word;
+      }
     }
   }
 }
 
-int grid_for(int64_t work, int threads) {
-  return static_cast<int>(std::min<int64_t>((work + threads - 1) / threads, static_cast<int64_t>(sm_count()) * 16));
+__global__ void __launch_bounds__(256)
+    mx4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                          bf16* __restrict__ out, int rows, int cols) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16;
+  const int lane = threadIdx.x % 16;
+  const int col_tiles = cols / 128;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  if (row >= rows) return;
+  const uint32_t* const scale_row = reinterpret_cast<const uint32_t*>(scales) +
+                                    (row / 128 * col_tiles) * 128 + (row % 32) * 4 + row / 32 % 4;
+  for (int t0 = blockIdx.y * kTiles; t0 < col_tiles; t0 += gridDim.y * kTiles) {
+    uint32_t q[kTiles], s[kTiles];
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) {
+      const bool own = t0 + j < col_tiles;
+      q[j] = own ? *reinterpret_cast<const uint32_t*>(codes + row * (cols / 2) + (t0 + j) * 64 + lane * 4) : 0u;
+      s[j] = own ? scale_row[static_cast<int64_t>(t0 + j) * 128] : 0u;
+    }
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) {
+      if (t0 + j >= col_tiles) break;
+      const uint4 v = mx4_expand_ordered(q[j], s[j] >> (8 * (lane / 4)) & 255u);
+      *reinterpret_cast<uint4*>(out + row * cols + (t0 + j) * 128 + lane * 8) = v;
+    }
+  }
 }
 
 }  // namespace
 
 void mx4_quantize(const bf16* x, uint8_t* codes, uint8_t* scales, int rows, int cols, cudaStream_t s) {
-  const int64_t work = static_cast<int64_t>((rows + 127) / 128 * 128) * (cols / 32);
-  mx4_quantize_kernel<<<grid_for(work, 256), 256, 0, s>>>(x, codes, scales, rows, cols);
-  check_cuda(cudaGetLastError(), "quantize_mxfp4 launch");
+  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(rows) + 127) / 128 * 8),
+                  static_cast<unsigned>(std::min((cols / 128 + kTiles - 1) / kTiles, 65535)));
+  launch(mx4_quantize_kernel, grid, 256, 0, 0, s, x, codes, scales, rows, cols);
 }
 
 void mx4_dequantize(const uint8_t* codes, const uint8_t* scales, bf16* out, int rows, int cols,
                     cudaStream_t s) {
-  const int64_t work = static_cast<int64_t>(rows) * (cols / 32);
-  mx4_dequantize_kernel<<<grid_for(work, 256), 256, 0, s>>>(codes, scales, out, rows, cols);
-  check_cuda(cudaGetLastError(), "dequantize_mxfp4 launch");
+  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(rows) + 15) / 16),
+                  static_cast<unsigned>(std::min((cols / 128 + kTiles - 1) / kTiles, 65535)));
+  launch(mx4_dequantize_kernel, grid, 256, 0, 0, s, codes, scales, out, rows, cols);
 }
 
 }  // namespace ce4b

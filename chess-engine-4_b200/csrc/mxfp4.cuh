@@ -39,6 +39,24 @@ __device__ __forceinline__ void mx4_expand(uint32_t w, uint32_t factor, uint32_t
   v[3] = mul_bf16x2(((w8 & 0x00F000F0u) * 0x0104u) & 0x81C081C0u, factor);
 }
 
+// Codes 0..7 of a word in order. A table of the eight scaled magnitudes is split into low and
+// high bytes; a byte permute looks up four codes at once (its selector nibbles are the codes
+// themselves), the sign bits are merged into the high bytes, and two more permutes interleave.
+__device__ __forceinline__ uint4 mx4_expand_ordered(uint32_t w, uint32_t scale) {
+  uint32_t f = scale * 0x00800080u;        // 2^(scale - 127), twice
+  if (scale == 0u) f = 0x00400040u;        // subnormal
+  if (scale == 255u) f = 0x7FFF7FFFu;      // NaN
+  const uint32_t p0 = mul_bf16x2(0x3F000000u, f), p1 = mul_bf16x2(0x3FC03F80u, f);  // 0, 0.5, 1, 1.5
+  const uint32_t p2 = mul_bf16x2(0x40404000u, f), p3 = mul_bf16x2(0x40C04080u, f);  // 2, 3, 4, 6
+  const uint32_t lo0 = prmt(p0, p1, 0x6420u), lo1 = prmt(p2, p3, 0x6420u);
+  const uint32_t hi0 = prmt(p0, p1, 0x7531u), hi1 = prmt(p2, p3, 0x7531u);
+  const uint32_t m = w & 0x77777777u, m4 = m >> 16, u = w << 4;
+  const uint32_t l0 = prmt(lo0, lo1, m), l1 = prmt(lo0, lo1, m4);
+  const uint32_t h0 = prmt(hi0, hi1, m) | (prmt(u, w, 0x5140u) & 0x80808080u);
+  const uint32_t h1 = prmt(hi0, hi1, m4) | (prmt(u, w, 0x7362u) & 0x80808080u);
+  return make_uint4(prmt(l0, h0, 0x5140u), prmt(l0, h0, 0x7362u), prmt(l1, h1, 0x5140u), prmt(l1, h1, 0x7362u));
+}
+
 // Columns 0..7 of a 16-byte chunk of x in the order of mx4_expand.
 __device__ __forceinline__ uint4 permute_x(const uint4& v) {
   return make_uint4(prmt(v.x, v.z, 0x5410u), prmt(v.x, v.z, 0x7632u), prmt(v.y, v.w, 0x5410u),

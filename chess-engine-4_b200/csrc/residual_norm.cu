@@ -18,47 +18,81 @@ namespace {
 // neighbours. Every form of the operator gives the same n, and the MXFP8 form quantises
 // exactly that value.
 struct RowScale {
-  float hi, lo;
+  float power;   // 2^e, about the factor's size
+  float hi, lo;  // factor / 2^e = hi + lo, lo >= 0
 };
 
 __device__ __forceinline__ RowScale row_scale(double sum, double inv_width, float eps) {
   const double f = rsqrt(fma(sum, inv_width, static_cast<double>(eps)));
   RowScale r;
-  r.hi = static_cast<float>(f);
-  r.lo = static_cast<float>(f - static_cast<double>(r.hi));
+  if (f > 0.0 && f <= 3.0e300) {
+    const int e = min(static_cast<int>((__double2hiint(f) >> 20) & 0x7FF) - 1023, 127);
+    const double m = f * __hiloint2double((1023 - e) << 20, 0);
+    r.power = static_cast<float>(__hiloint2double((1023 + e) << 20, 0));
+    r.hi = __double2float_rz(m);
+    // Never 0: a product that overflows stays infinite when multiplied by it.
+    r.lo = fmaxf(static_cast<float>(m - static_cast<double>(r.hi)), 0x1p-60f);
+  } else {  // 0 beside an infinity, infinite for a row of zeros without eps, NaN
+    r.power = static_cast<float>(f);
+    r.hi = 1.0f;
+    r.lo = 0x1p-60f;
+  }
   return r;
 }
 
-// s * (hi + lo) * w: q is the FP32 rounding of the product and e the rest, so that q + e is the
-// product rounded to FP32 once (about 2^-46 of it is lost before). An overflowing q has no rest.
+// s * factor * w rounded to FP32 once. s * 2^e is exact and of the size of s * factor, so its
+// product with w (eight bits each: exact) overflows only where the result does; the last FMA
+// rounds the exact p * hi plus p * lo.
 __device__ __forceinline__ float scale_product(float s, float w, const RowScale& f) {
-  const float t = s * f.hi;
-  const float te = fmaf(s, f.lo, fmaf(s, f.hi, -t));
-  const float q = t * w;
-  const float e = fmaf(te, w, fmaf(t, w, -q));
-  return fabsf(q) <= 3.0e38f ? q + e : q;
+  const float p = s * f.power * w;
+  return fmaf(p, f.hi, p * f.lo);
 }
 
-__device__ __forceinline__ double warp_sum(double v) {
+// Sum over each group of WIDTH lanes.
+template <int WIDTH>
+__device__ __forceinline__ double lane_sum(double v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = WIDTH / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// Eight BF16 values of a row: a 16-byte access where the whole chunk belongs to the row, single
-// elements at the ends of rows that do not start or end on 16 bytes. `from`..`to` are the
-// chunk's elements that the row owns.
-__device__ __forceinline__ uint4 load_chunk(const bf16* p, int from, int to) {
-  if (from == 0 && to == 8) return *reinterpret_cast<const uint4*>(p);
-  uint32_t v[4] = {};
-  const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
+// Elements from..to-1 of a chunk of eight, the others 0.
+__device__ __forceinline__ uint4 keep(const uint4& q, int from, int to) {
+  uint32_t v[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (j >= from && j < to) v[j / 2] |= static_cast<uint32_t>(u[j]) << (16 * (j % 2));
+  for (int j = 0; j < 4; ++j) {
+    if (2 * j < from || 2 * j >= to) v[j] &= 0xFFFF0000u;
+    if (2 * j + 1 < from || 2 * j + 1 >= to) v[j] &= 0x0000FFFFu;
   }
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+// The chunk of eight BF16 values at p, of which `limit` exist (at least one): a 16-byte load,
+// or single elements at the end of the buffer.
+__device__ __forceinline__ uint4 load_chunk(const bf16* p, int64_t limit) {
+  if (limit >= 8) return *reinterpret_cast<const uint4*>(p);
+  uint32_t v[4] = {};
+  const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (j < limit) v[j / 2] |= static_cast<uint32_t>(u[j]) << (16 * (j % 2));
+  }
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// Elements o..o+7 (o = 0..7) of the sixteen of a and b.
+__device__ __forceinline__ uint4 window(const uint4& a, const uint4& b, int o) {
+  uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int j = 0; j < 6; ++j) v[j] = o & 4 ? v[j + 2] : v[j];
+#pragma unroll
+  for (int j = 0; j < 5; ++j) v[j] = o & 2 ? v[j + 1] : v[j];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = o & 1 ? __funnelshift_r(v[j], v[j + 1], 16) : v[j];
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// Stores elements from..to-1 of a chunk; a neighbouring row owns the others.
 __device__ __forceinline__ void store_chunk(bf16* p, const uint32_t (&v)[4], int from, int to) {
   if (from == 0 && to == 8) {
     *reinterpret_cast<uint4*>(p) = make_uint4(v[0], v[1], v[2], v[3]);
@@ -74,7 +108,8 @@ __device__ __forceinline__ void store_chunk(bf16* p, const uint32_t (&v)[4], int
 // A row is held in the registers of TPR threads, V chunks of eight columns each, and read and
 // written once. ALIGNED: rows start and end on 16 bytes (width % 8 == 0), and a thread keeps
 // its part of w over the rows it takes. Otherwise chunks are the aligned 16 bytes of the
-// matrix, and the row's first and last one are accessed by elements.
+// matrix: the row's first and last one hold elements of its neighbours, which are masked
+// after the load and left out of the store, and w is shifted to the row's offset.
 template <int V, int TPR, bool ALIGNED, bool MX>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
     add_rmsnorm_kernel(const bf16* x, const bf16* residual, const bf16* __restrict__ w, bf16* sum,
@@ -82,19 +117,29 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
                        double inv_width, float eps) {
   constexpr int kThreads = TPR > 256 ? TPR : 256;
   constexpr int kRows = kThreads / TPR;  // rows of a block at a time
-  constexpr int kWarps = TPR / 32;       // warps of a row
+  constexpr int kWarps = TPR < 32 ? 1 : TPR / 32;  // warps of a row
   __shared__ double part[2][kThreads / 32];
   const int lane = threadIdx.x % TPR;
   grid_dependency_wait();
   grid_launch_dependents();
+  // w is loaded ahead of the row's sum, or, where registers are short, at its use.
+  constexpr bool kKeepW = V <= 2 || (ALIGNED && V <= 4);
+  auto load_w = [&](int c, int shift) {  // columns c - shift .. + 7 of w
+    if constexpr (ALIGNED) return *reinterpret_cast<const uint4*>(w + c);
+    uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
+    if (shift > 0 && c > 0) a = load_chunk(w + c - 8, width - c + 8);
+    if (c < width) b = load_chunk(w + c, width - c);
+    return shift > 0 ? window(a, b, 8 - shift) : b;
+  };
   uint4 wv[V];
-  if constexpr (ALIGNED) {
+  if constexpr (ALIGNED && kKeepW) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int c = (i * TPR + lane) * 8;
       wv[i] = c < width ? *reinterpret_cast<const uint4*>(w + c) : make_uint4(0u, 0u, 0u, 0u);
     }
   }
+  const int64_t total = static_cast<int64_t>(rows) * width;
   const int last = MX ? (rows + 127) / 128 * 128 : rows;
   int turn = 0;
   for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * kRows; r0 < last;
@@ -118,8 +163,25 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
       const bool own = bounds(i, from, to);
       const int64_t at = begin + (i * TPR + lane) * 8;
       v[i] = r[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (own) v[i] = load_chunk(x + at, from, to);
-      if (own && residual != nullptr) r[i] = load_chunk(residual + at, from, to);
+      if constexpr (ALIGNED) {
+        if (own) v[i] = *reinterpret_cast<const uint4*>(x + at);
+        if (own && residual != nullptr) r[i] = *reinterpret_cast<const uint4*>(residual + at);
+      } else if (own) {
+        v[i] = load_chunk(x + at, total - at);
+        if (residual != nullptr) r[i] = load_chunk(residual + at, total - at);
+        if (from > 0 || to < 8) {
+          v[i] = keep(v[i], from, to);
+          r[i] = keep(r[i], from, to);
+        }
+      }
+    }
+    if constexpr (!ALIGNED && kKeepW) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        int from, to;
+        wv[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (bounds(i, from, to)) wv[i] = load_w((i * TPR + lane) * 8, shift);
+      }
     }
     double ss = 0.0;
 #pragma unroll
@@ -144,7 +206,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
         store_chunk(sum + begin + (i * TPR + lane) * 8, words, from, to);
       }
     }
-    ss = warp_sum(ss);
+    ss = lane_sum<TPR < 32 ? TPR : 32>(ss);
     if constexpr (kWarps > 1) {
       const int warp = threadIdx.x / 32;
       if (threadIdx.x % 32 == 0) part[turn][warp] = ss;
@@ -161,17 +223,16 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
       const uint32_t* q = reinterpret_cast<const uint32_t*>(&v[i]);
       const int c = (i * TPR + lane) * 8;
       float n[8];
+      uint4 wi = make_uint4(0u, 0u, 0u, 0u);
+      if constexpr (kKeepW) {
+        wi = wv[i];
+      } else if (own) {
+        wi = load_w(c, shift);
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 s = unpack_bf16x2(q[j]);
-        float2 u;
-        if constexpr (ALIGNED) {
-          u = unpack_bf16x2(reinterpret_cast<const uint32_t*>(&wv[i])[j]);
-        } else {
-          const int col = c - shift + 2 * j;
-          u.x = own && 2 * j >= from && 2 * j < to ? __bfloat162float(w[col]) : 0.0f;
-          u.y = own && 2 * j + 1 >= from && 2 * j + 1 < to ? __bfloat162float(w[col + 1]) : 0.0f;
-        }
+        const float2 u = unpack_bf16x2(reinterpret_cast<const uint32_t*>(&wi)[j]);
         n[2 * j] = scale_product(s.x, u.x, f);
         n[2 * j + 1] = scale_product(s.y, u.y, f);
       }
@@ -219,15 +280,26 @@ __global__ void add_rmsnorm_any_kernel(const bf16* x, const bf16* residual, cons
   }
   const size_t at = static_cast<size_t>(row) * width;
   double ss = 0.0;
-  for (int c = threadIdx.x; c < width; c += blockDim.x) {
-    float s = __bfloat162float(x[at + c]);
-    if (residual != nullptr) {
-      s = bf16_round(s + __bfloat162float(residual[at + c]));
-      sum[at + c] = __float2bfloat16_rn(s);
+  const int step = blockDim.x;
+  for (int c0 = threadIdx.x; c0 < width; c0 += 4 * step) {
+    float s[4], r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = c0 + j * step;
+      s[j] = c < width ? __bfloat162float(x[at + c]) : 0.0f;
+      r[j] = c < width && residual != nullptr ? __bfloat162float(residual[at + c]) : 0.0f;
     }
-    ss = fma(static_cast<double>(s), static_cast<double>(s), ss);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = c0 + j * step;
+      if (residual != nullptr && c < width) {
+        s[j] = bf16_round(s[j] + r[j]);
+        sum[at + c] = __float2bfloat16_rn(s[j]);
+      }
+      ss = fma(static_cast<double>(s[j]), static_cast<double>(s[j]), ss);
+    }
   }
-  ss = warp_sum(ss);
+  ss = lane_sum<32>(ss);
   if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = ss;
   __syncthreads();  // also before the sum of other threads' columns is read below
   ss = 0.0;
@@ -235,7 +307,8 @@ __global__ void add_rmsnorm_any_kernel(const bf16* x, const bf16* residual, cons
   const RowScale f = row_scale(ss, inv_width, eps);
   const bf16* src = residual != nullptr ? sum : x;
   if (codes == nullptr) {
-    for (int c = threadIdx.x; c < width; c += blockDim.x) {
+#pragma unroll 4
+    for (int c = threadIdx.x; c < width; c += step) {
       out[at + c] = __float2bfloat16_rn(
           scale_product(__bfloat162float(src[at + c]), __bfloat162float(w[c]), f));
     }
@@ -281,6 +354,8 @@ bool launch_rows(const NormArgs& a) {
   // chunks a thread, so that a row is a warp's or few warps' business and its sum needs few
   // steps across warps.
   const bool few = static_cast<int64_t>(a.rows) * chunks <= static_cast<int64_t>(sm_count()) * 2048;
+  if (chunks <= 8) return launch_norm<1, 8, ALIGNED, MX>(a), true;
+  if (chunks <= 16) return launch_norm<1, 16, ALIGNED, MX>(a), true;
   if (few && chunks <= 1024) {
     if (chunks <= 32) return launch_norm<1, 32, ALIGNED, MX>(a), true;
     if (chunks <= 64) return launch_norm<1, 64, ALIGNED, MX>(a), true;
@@ -291,11 +366,12 @@ bool launch_rows(const NormArgs& a) {
   }
   if (chunks <= 32) return launch_norm<1, 32, ALIGNED, MX>(a), true;
   if (chunks <= 64) return launch_norm<2, 32, ALIGNED, MX>(a), true;
-  if (chunks <= 128) return launch_norm<4, 32, ALIGNED, MX>(a), true;
-  if (chunks <= 256) return launch_norm<4, 64, ALIGNED, MX>(a), true;
-  if (chunks <= 512) return launch_norm<4, 128, ALIGNED, MX>(a), true;
-  if (chunks <= 1024) return launch_norm<4, 256, ALIGNED, MX>(a), true;
-  if (chunks <= 2048) return launch_norm<4, 512, ALIGNED, MX>(a), true;
+  if (chunks <= 128) return ALIGNED ? launch_norm<2, 64, ALIGNED, MX>(a) : launch_norm<4, 32, ALIGNED, MX>(a), true;
+  if (chunks <= 256) return ALIGNED ? launch_norm<2, 128, ALIGNED, MX>(a) : launch_norm<4, 64, ALIGNED, MX>(a), true;
+  if (chunks <= 512) return ALIGNED ? launch_norm<2, 256, ALIGNED, MX>(a) : launch_norm<4, 128, ALIGNED, MX>(a), true;
+  if (chunks <= 1024) return ALIGNED ? launch_norm<2, 512, ALIGNED, MX>(a) : launch_norm<4, 256, ALIGNED, MX>(a), true;
+  if (chunks <= 2048) return launch_norm<2, 1024, ALIGNED, MX>(a), true;
+  if (chunks <= 4096) return launch_norm<8, 512, ALIGNED, MX>(a), true;
   return false;
 }
 
@@ -307,14 +383,14 @@ void add_rmsnorm_rows(const bf16* x, const bf16* residual, const bf16* w, bf16* 
   const NormArgs a{x, residual, w, sum, out, codes, scales, rows, width, eps, s};
   auto wide = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
   const bool mx = codes != nullptr;
-  if (wide(x) && wide(residual) && (residual == nullptr || wide(sum)) && (mx || wide(out))) {
-    const bool aligned = width % 8 == 0 && wide(w);
-    if (mx ? aligned && launch_rows<true, true>(a) : aligned ? launch_rows<true, false>(a) : launch_rows<false, false>(a)) {
+  if (wide(x) && wide(residual) && wide(w) && (residual == nullptr || wide(sum)) && (mx || wide(out))) {
+    const bool aligned = width % 8 == 0;
+    if (mx ? launch_rows<true, true>(a) : aligned ? launch_rows<true, false>(a) : launch_rows<false, false>(a)) {
       return;
     }
   }
   const int grid = mx ? (rows + 127) / 128 * 128 : rows;
-  add_rmsnorm_any_kernel<<<grid, 256, 0, s>>>(x, residual, w, sum, out, codes, scales, rows, width,
+  add_rmsnorm_any_kernel<<<grid, width > 4096 ? 1024 : 256, 0, s>>>(x, residual, w, sum, out, codes, scales, rows, width,
                                               1.0 / width, eps);
   check_cuda(cudaGetLastError(), "add_rmsnorm launch");
 }

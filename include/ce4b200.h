@@ -454,12 +454,13 @@ int ce4b_add_rmsnorm_mxfp8(const void* x_dev, const void* residual_dev, const vo
  * [ceil(rows/128), cols/128, 32, 16] in the layout of ce4b_quantize_mxfp8 (padding rows 0).
  * scale = the smallest power of two, at least 2^-39, that leaves no magnitude of its 32
  * columns over 6; codes = round-to-nearest-even of x / scale. A group with a NaN or an
- * infinity gets scale 255, which stands for NaN. x and codes are 16-byte aligned. */
+ * infinity gets scale 255, which stands for NaN. x, codes and scales are
+ * 16-byte aligned. */
 int ce4b_quantize_mxfp4(const void* x_dev, void* codes_dev, void* scales_dev, int rows, int cols,
                         void* stream);
 
 /* The BF16 values [rows, cols] that MXFP4 codes and scales stand for (exact where BF16 holds
- * them: magnitudes below 2^128). codes and out are 16-byte aligned. */
+ * them: magnitudes below 2^128). codes, scales and out are 16-byte aligned. */
 int ce4b_dequantize_mxfp4(const void* codes_dev, const void* scales_dev, void* out_dev, int rows,
                           int cols, void* stream);
 

@@ -135,6 +135,8 @@ def test_c_entries_check_on_the_host() -> None:
     refused(lib.ce4b_quantize_mxfp4(p, p, None, 1, 128, None), "null")
     refused(lib.ce4b_quantize_mxfp4(p, p, p, 1, 96, None), "multiple of 128")
     refused(lib.ce4b_quantize_mxfp4(p + 2, p, p, 1, 128, None), "aligned")
+    refused(lib.ce4b_quantize_mxfp4(p, p, p + 4, 1, 128, None), "aligned")
+    refused(lib.ce4b_dequantize_mxfp4(p, p + 4, p, 1, 128, None), "aligned")
     refused(lib.ce4b_dequantize_mxfp4(p, p, p, -1, 128, None), "positive")
     refused(lib.ce4b_dequantize_mxfp4(p, p, p + 2, 1, 128, None), "aligned")
     refused(lib.ce4b_mxfp4_linear(p, p, p, None, None, 1, 8, 128, None), "null")
