@@ -126,13 +126,18 @@ def _check_extents(tensor: torch.Tensor) -> None:
 
 
 # The operators below are called once per layer on batches of a few rows, where the host's
-# time per call is the call's time: what is as it should be is recognised by a few cheap
-# tests, and the checks that word an error run only if one of those fails.
+# time per call is the call's time: operands that are as they should be pass one cheap test,
+# and the checks that word an error run only if it fails.
+def _is_bf16_matrix(tensor: torch.Tensor) -> bool:
+    if not (tensor.is_cuda and tensor.dtype is torch.bfloat16 and tensor.is_contiguous()):
+        return False
+    shape = tensor.shape
+    return len(shape) == 2 and 1 <= shape[0] <= _MAX_EXTENT and 1 <= shape[1] <= _MAX_EXTENT
+
+
 def _need_bf16_matrix(name: str, tensor: torch.Tensor) -> None:
-    if not (tensor.is_cuda and tensor.dtype is torch.bfloat16 and tensor.dim() == 2 and tensor.is_contiguous()):
+    if not _is_bf16_matrix(tensor):
         _check_bf16_matrix(name, tensor)
-    rows, cols = tensor.shape
-    if not (1 <= rows <= _MAX_EXTENT and 1 <= cols <= _MAX_EXTENT):
         _check_extents(tensor)
 
 
@@ -140,11 +145,10 @@ def _same_device(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.get_device() == b.get_device() if a.is_cuda and b.is_cuda else a.device == b.device
 
 
-def _call(name: str, tensor: torch.Tensor, *args: object) -> None:
-    """Call a C entry (its last argument is the stream) on `tensor`'s device and stream."""
+def _call(name: str, index: int, *args: object) -> None:
+    """Call a C entry (its last argument is the stream) on device `index` and its stream."""
 
     fn = getattr(_lib.library(), name)
-    index = tensor.get_device()
     if index == torch._C._cuda_getDevice():
         status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
@@ -154,9 +158,19 @@ def _call(name: str, tensor: torch.Tensor, *args: object) -> None:
         _lib.check(status)
 
 
-def _check_norm_operands(
+def _need_norm_operands(
     x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor
 ) -> None:
+    if _is_bf16_matrix(x) and weight.is_cuda and weight.dtype is torch.bfloat16:
+        shape, index = x.shape, x.get_device()
+        if (
+            weight.shape == shape[1:] and weight.is_contiguous() and weight.get_device() == index
+            and (residual is None or (
+                residual.is_cuda and residual.dtype is torch.bfloat16 and residual.is_contiguous()
+                and residual.shape == shape and residual.get_device() == index
+            ))
+        ):
+            return
     _need_bf16_matrix("x", x)
     if residual is not None:
         _need_bf16_matrix("residual", residual)
@@ -164,8 +178,7 @@ def _check_norm_operands(
             raise ValueError("residual must match x")
         if not _same_device(residual, x):
             raise ValueError("residual must be on x's device")
-    if not (weight.is_cuda and weight.dtype is torch.bfloat16 and weight.shape == x.shape[1:] and weight.is_contiguous()):
-        _check_bf16_vector("weight", weight, x.shape[1])
+    _check_bf16_vector("weight", weight, x.shape[1])
     if not _same_device(weight, x):
         raise ValueError("weight must be on x's device")
 
@@ -182,11 +195,13 @@ def add_rmsnorm_forward(
     returned as the sum. BF16 rows of any width.
     """
 
-    _check_norm_operands(x, residual, weight)
+    _need_norm_operands(x, residual, weight)
     out = torch.empty_like(x)
     total = x if residual is None else torch.empty_like(x)
     _call(
-        "ce4b_add_rmsnorm", x, x.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(), total.data_ptr(), out.data_ptr(), x.shape[0], x.shape[1], eps,
+        "ce4b_add_rmsnorm", x.get_device(), x.data_ptr(),
+        None if residual is None else residual.data_ptr(), weight.data_ptr(), total.data_ptr(),
+        out.data_ptr(), x.shape[0], x.shape[1], eps,
     )
     return total, out
 
@@ -201,7 +216,7 @@ def add_rmsnorm_mxfp8(
     rows with zero bytes, and :func:`mxfp8_gemm` takes such a left operand).
     """
 
-    _check_norm_operands(x, residual, weight)
+    _need_norm_operands(x, residual, weight)
     rows, width = x.shape
     if width % MXFP8_TILE_SIZE:
         raise ValueError(f"x must have a multiple of {MXFP8_TILE_SIZE} columns")
@@ -209,7 +224,9 @@ def add_rmsnorm_mxfp8(
     scales = torch.empty(-(-rows // 128), width // 128, 32, 16, dtype=torch.uint8, device=x.device)
     total = x if residual is None else torch.empty_like(x)
     _call(
-        "ce4b_add_rmsnorm_mxfp8", x, x.data_ptr(), None if residual is None else residual.data_ptr(), weight.data_ptr(), total.data_ptr(), values.data_ptr(), scales.data_ptr(), rows, width, eps,
+        "ce4b_add_rmsnorm_mxfp8", x.get_device(), x.data_ptr(),
+        None if residual is None else residual.data_ptr(), weight.data_ptr(), total.data_ptr(),
+        values.data_ptr(), scales.data_ptr(), rows, width, eps,
     )
     return total, Mxfp8Tensor(values=values, scales=scales)
 
@@ -430,7 +447,8 @@ def quantize_mxfp4(weight: torch.Tensor) -> Mxfp4Tensor:
     values = torch.empty(rows, cols // 2, dtype=torch.uint8, device=weight.device)
     scales = torch.empty(-(-rows // 128), cols // 128, 32, 16, dtype=torch.uint8, device=weight.device)
     _call(
-        "ce4b_quantize_mxfp4", weight, weight.data_ptr(), values.data_ptr(), scales.data_ptr(), rows, cols,
+        "ce4b_quantize_mxfp4", weight.get_device(), weight.data_ptr(), values.data_ptr(),
+        scales.data_ptr(), rows, cols,
     )
     return Mxfp4Tensor(values=values, scales=scales)
 
@@ -442,7 +460,8 @@ def dequantize_mxfp4(weight: Mxfp4Tensor) -> torch.Tensor:
     values = weight.values
     out = torch.empty(rows, cols, dtype=torch.bfloat16, device=values.device)
     _call(
-        "ce4b_dequantize_mxfp4", values, values.data_ptr(), weight.scales.data_ptr(), out.data_ptr(), rows, cols,
+        "ce4b_dequantize_mxfp4", values.get_device(), values.data_ptr(), weight.scales.data_ptr(),
+        out.data_ptr(), rows, cols,
     )
     return out
 
@@ -466,7 +485,9 @@ def mxfp4_linear(
             raise ValueError(f"residual must have shape [{rows}, {n}] on x's device")
     out = x.new_empty(rows, n)
     _call(
-        "ce4b_mxfp4_linear", x, x.data_ptr(), weight.values.data_ptr(), weight.scales.data_ptr(), None if residual is None else residual.data_ptr(), out.data_ptr(), rows, n, k,
+        "ce4b_mxfp4_linear", x.get_device(), x.data_ptr(), weight.values.data_ptr(),
+        weight.scales.data_ptr(), None if residual is None else residual.data_ptr(),
+        out.data_ptr(), rows, n, k,
     )
     return out
 
@@ -485,7 +506,8 @@ def mxfp4_swiglu(x: torch.Tensor, gate_up_weight: Mxfp4Tensor) -> torch.Tensor:
         raise ValueError("gate_up_weight must have an even number of rows")
     hidden = x.new_empty(rows, wide // 2)
     _call(
-        "ce4b_mxfp4_swiglu", x, x.data_ptr(), gate_up_weight.values.data_ptr(), gate_up_weight.scales.data_ptr(), hidden.data_ptr(), rows, wide // 2, k,
+        "ce4b_mxfp4_swiglu", x.get_device(), x.data_ptr(), gate_up_weight.values.data_ptr(),
+        gate_up_weight.scales.data_ptr(), hidden.data_ptr(), rows, wide // 2, k,
     )
     return hidden
 
