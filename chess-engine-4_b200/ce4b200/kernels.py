@@ -328,7 +328,7 @@ class Mxfp8Tensor:
     """E4M3 codes and their E8M0 scale tiles (src/chess_engine_4/kernels/dense.py:27-30)."""
 
     values: torch.Tensor  # float8_e4m3fn [rows, cols]
-    scales: torch.Tensor  # uint8 [rows/128, cols/128, 32, 16]
+    scales: torch.Tensor  # uint8 [ceil(rows/128), cols/128, 32, 16]
 
 
 def _check_mx_matrix(name: str, tensor: torch.Tensor) -> None:
@@ -372,7 +372,9 @@ def quantize_mxfp8_transpose(tensor: torch.Tensor) -> Mxfp8Tensor:
 
 def mxfp8_gemm(left: Mxfp8Tensor, right: Mxfp8Tensor) -> torch.Tensor:
     """``dequant(left) @ dequant(right).T`` in BF16 on block-scaled tcgen05 MMAs
-    (replaces kernels/dense.py:87-113; any output width divisible by 128)."""
+    (replaces kernels/dense.py:87-113; any output width divisible by 128, and any number of
+    rows of ``left`` whose scale tiles are padded to 128 rows, as :func:`add_rmsnorm_mxfp8`
+    writes them)."""
 
     rows, reduction = left.values.shape
     out_cols, right_reduction = right.values.shape
@@ -381,8 +383,10 @@ def mxfp8_gemm(left: Mxfp8Tensor, right: Mxfp8Tensor) -> torch.Tensor:
     for t in (left.values, right.values):
         if t.device.type != "cuda" or t.dtype != torch.float8_e4m3fn or not t.is_contiguous():
             raise ValueError("MXFP8 values must be contiguous float8_e4m3fn CUDA tensors")
-    if rows % 128 or out_cols % 128 or reduction % 128:
-        raise ValueError("MXFP8 GEMM dimensions must be multiples of 128")
+    if rows < 1 or out_cols % 128 or reduction % 128:
+        raise ValueError("MXFP8 GEMM columns and reduction must be multiples of 128")
+    if rows % 128 and left.scales.shape != (-(-rows // 128), reduction // 128, 32, 16):
+        raise ValueError("MXFP8 scale tiles of a ragged operand must be padded to 128 rows")
     out = torch.empty(rows, out_cols, dtype=torch.bfloat16, device=left.values.device)
     with torch.cuda.device(out.device):
         _lib.check(

@@ -581,9 +581,8 @@ int ce4b_mxfp8_gemm(const void* a_codes_dev, const void* a_scales_dev, const voi
                     const void* b_scales_dev, void* c_dev, int m, int n, int k, void* stream) {
   return guarded([&] {
     require(a_codes_dev && a_scales_dev && b_codes_dev && b_scales_dev && c_dev, "null pointer");
-    require(m >= 128 && n >= 128 && k >= 128, "MXFP8 GEMM extents must be at least 128");
-    require(m % 128 == 0 && n % 128 == 0 && k % 128 == 0,
-            "MXFP8 GEMM extents must be multiples of 128");
+    require(m >= 1 && n >= 128 && k >= 128, "MXFP8 GEMM N and K must be at least 128");
+    require(n % 128 == 0 && k % 128 == 0, "MXFP8 GEMM N and K must be multiples of 128");
     const CUtensorMap ta = make_tmap_u8(a_codes_dev, m, k, k, 128);
     const CUtensorMap tb = make_tmap_u8(b_codes_dev, n, k, k, 128);
     const CUtensorMap tc = make_tmap_bf16(c_dev, m, n, n, 128);

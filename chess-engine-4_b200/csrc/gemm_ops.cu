@@ -158,14 +158,13 @@ CUtensorMap make_tmap_u8_sw64(const void* ptr, uint64_t rows, uint64_t cols, uin
 void gemm_mx_store_bf16(const CUtensorMap& tA, const CUtensorMap& tB, const CUtensorMap& tC,
                         const uint8_t* sfa, const uint8_t* sfb, int m, int n, int k,
                         cudaStream_t s) {
-  require(m % 128 == 0 && n % 128 == 0 && k % 128 == 0,
-          "MXFP8 GEMM extents must be multiples of 128");
+  require(n % 128 == 0 && k % 128 == 0, "MXFP8 GEMM N and K must be multiples of 128");
   constexpr int BN = 128, NS = 5, NA = 2;
   using Epi = EpiStoreBF16<BN>;
   auto kernel = gemm_mx_kernel<BN, NS, NA, 1, kG, false, DenseSched, Epi>;
   constexpr int smem = GemmMxSmem<BN, NS, NA, Epi>::kBytes;
   ensure_smem(kernel, smem);
-  DenseSched sched{m, n / BN, (m / kBM) * (n / BN), BN, 0};
+  DenseSched sched{m, n / BN, ceil_div(m, kBM) * (n / BN), BN, 0};
   typename Epi::Params ep{n};
   const MxScales sf{sfa, sfb, k / 128};
   const int grid = std::min(sched.num_tiles, sm_count());

@@ -132,7 +132,8 @@ CUtensorMap make_tmap_u8(const void* ptr, uint64_t rows, uint64_t cols, uint64_t
 // Same with a 64-byte swizzle and box = 64 bytes x box_rows.
 CUtensorMap make_tmap_u8_sw64(const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld_bytes,
                               uint32_t box_rows);
-// C[M,N] BF16 = block-scaled E4M3 A[M,K] . B[N,K]^T (M, N, K multiples of 128; maps with
+// C[M,N] BF16 = block-scaled E4M3 A[M,K] . B[N,K]^T (N, K multiples of 128, A's scale
+// tiles padded to 128 rows; maps with
 // 128-row boxes; C map BF16 with 128-row boxes).
 void gemm_mx_store_bf16(const CUtensorMap& tA, const CUtensorMap& tB, const CUtensorMap& tC,
                         const uint8_t* sfa, const uint8_t* sfb, int m, int n, int k,

@@ -154,3 +154,42 @@ def test_graph_replay_reads_new_inputs() -> None:
     assert torch.equal(total, want_total) and torch.equal(n, want_n) and torch.equal(total8, want_total8)
     assert torch.equal(q.values.view(torch.uint8), want_q.values.view(torch.uint8))
     assert torch.equal(q.scales, want_q.scales)
+
+
+@pytest.mark.parametrize("rows,d,h", [(1, 256, 512), (77, 512, 1536), (128, 256, 768), (300, 512, 1024)])
+def test_mxfp8_blocks_of_a_ragged_batch(rows: int, d: int, h: int) -> None:
+    """Two MXFP8 products as a tower chains them: the norm's codes feed the block-scaled GEMM
+    with any number of rows, and the next norm adds the product to the stream. Each product
+    is compared with the 64-bit product of the dequantised operands: one BF16 rounding (2^-8)
+    and FP32 sums of K / 32 steps, each off by at most 2^-22 of the sum of magnitudes."""
+
+    from ce4b200 import kernels
+    from oracle import mxfp8
+
+    g = torch.Generator().manual_seed(rows + d)
+    x, residual, weight = _inputs(rows, d, 4)
+    up = kernels.quantize_mxfp8((torch.randn(h, d, generator=g) / d**0.5).bfloat16().cuda())
+    down = kernels.quantize_mxfp8((torch.randn(d, h, generator=g) / h**0.5).bfloat16().cuda())
+    ones = torch.ones(h, dtype=torch.bfloat16, device="cuda")
+
+    def product(left, right):
+        got = kernels.mxfp8_gemm(left, right)
+        pad = -(-rows // 128) * 128
+        codes = torch.zeros(pad, left.values.shape[1], dtype=torch.uint8)
+        codes[:rows] = left.values.view(torch.uint8).cpu()
+        a = mxfp8.dequantize(codes, left.scales.cpu())[:rows].double()
+        b = mxfp8.dequantize(right.values.view(torch.uint8).cpu(), right.scales.cpu()).double()
+        ref, mags = a @ b.T, a.abs() @ b.abs().T
+        err = (got.double().cpu() - ref).abs()
+        assert bool((err <= ref.abs() * 2.0**-8 + mags * (b.shape[1] / 32 * 2.0**-22)).all())
+        return got
+
+    total, n = kernels.add_rmsnorm_mxfp8(x, residual, weight)
+    hidden = product(n, up)
+    _, hidden8 = kernels.add_rmsnorm_mxfp8(hidden, None, ones)
+    y = product(hidden8, down)
+    final, q = kernels.add_rmsnorm_mxfp8(y, total, weight)
+    assert torch.equal(final, (y.float() + total.float()).bfloat16())
+    assert q.values.shape == (rows, d)
+    with pytest.raises(ValueError, match="padded"):
+        kernels.mxfp8_gemm(kernels.Mxfp8Tensor(n.values[:1], n.scales[:0]), up)
