@@ -21,22 +21,34 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
 }
 
 // The factor 2^(scale - 1) of a group, twice in a register. It overflows BF16 from scale 129
-// (groups whose largest weight is over 12): there it is 2^127, and mx4_factor2 holds the rest.
+// (groups whose largest weight is over 12): mx4_wide_factor stops at 2^127 there, and
+// mx4_factor2 holds the rest. Scale 255 is NaN.
 __device__ __forceinline__ uint32_t mx4_factor(uint32_t scale) {
-  return scale == 255u ? 0x7FFF7FFFu : min(scale + 126u, 254u) * 0x00800080u;  // 255 is NaN
+  return scale * 0x00800080u + 126u * 0x00800080u;
+}
+
+__device__ __forceinline__ uint32_t mx4_wide_factor(uint32_t scale) {
+  return scale == 255u ? 0x7FFF7FFFu : min(scale + 126u, 254u) * 0x00800080u;
 }
 
 __device__ __forceinline__ uint32_t mx4_factor2(uint32_t scale) {
   return (scale > 128u && scale < 255u ? scale - 1u : 127u) * 0x00800080u;
 }
 
+// The two multipliers, kept from the compiler, which would turn a product into shifts and an
+// addition: the multiplication runs beside the ALU, which bounds the expansion.
+struct Mx4Spread {
+  uint32_t even = 0x1040u, odd = 0x0104u;
+  __device__ __forceinline__ Mx4Spread() { asm volatile("" : "+r"(even), "+r"(odd)); }
+};
+
 // Codes 0..7 of a word as (0, 4), (1, 5), (2, 6), (3, 7).
-__device__ __forceinline__ void mx4_expand(uint32_t w, uint32_t factor, uint32_t (&v)[4]) {
+__device__ __forceinline__ void mx4_expand(uint32_t w, uint32_t factor, const Mx4Spread& m, uint32_t (&v)[4]) {
   const uint32_t w8 = w >> 8;
-  v[0] = mul_bf16x2(((w & 0x000F000Fu) * 0x1040u) & 0x81C081C0u, factor);
-  v[1] = mul_bf16x2(((w & 0x00F000F0u) * 0x0104u) & 0x81C081C0u, factor);
-  v[2] = mul_bf16x2(((w8 & 0x000F000Fu) * 0x1040u) & 0x81C081C0u, factor);
-  v[3] = mul_bf16x2(((w8 & 0x00F000F0u) * 0x0104u) & 0x81C081C0u, factor);
+  v[0] = mul_bf16x2(((w & 0x000F000Fu) * m.even) & 0x81C081C0u, factor);
+  v[1] = mul_bf16x2(((w & 0x00F000F0u) * m.odd) & 0x81C081C0u, factor);
+  v[2] = mul_bf16x2(((w8 & 0x000F000Fu) * m.even) & 0x81C081C0u, factor);
+  v[3] = mul_bf16x2(((w8 & 0x00F000F0u) * m.odd) & 0x81C081C0u, factor);
 }
 
 // Codes 0..7 of a word in order. A table of the eight scaled magnitudes is split into low and
@@ -61,6 +73,15 @@ __device__ __forceinline__ uint4 mx4_expand_ordered(uint32_t w, uint32_t scale) 
 __device__ __forceinline__ uint4 permute_x(const uint4& v) {
   return make_uint4(prmt(v.x, v.z, 0x5410u), prmt(v.x, v.z, 0x7632u), prmt(v.y, v.w, 0x5410u),
                     prmt(v.y, v.w, 0x7632u));
+}
+
+// Weight bytes are read once: they leave the L1 cache to x.
+__device__ __forceinline__ uint4 load_stream(const uint8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
 }
 
 }  // namespace ce4b

@@ -1,21 +1,22 @@
-// Products of a few BF16 activation rows with an MXFP4 weight (kernel-op API mxfp4_linear,
+// Products of 17 and more BF16 activation rows with an MXFP4 weight (kernel-op API mxfp4_linear,
 // mxfp4_swiglu): y[r, n] = sum_k x[r, k] * code[n, k] * 2^(scale[n, k / 32] - 127).
 //
-// The time is the weight's 0.53 bytes per element, as long as turning codes into operands
-// keeps up with them: an SM takes in about 43 codes a clock at the memory's rate and issues
-// 128 lane operations, so a code may cost at most three, whatever is done with it. A multiply
-// per activation row would spend those on the first few rows. So the weight is the A operand
-// of tcgen05 MMAs (128 weight rows are the 128 lanes of tensor memory, up to 64 activation rows
-// the N columns): every code is expanded once, in registers, to the BF16 value it stands for
-// (E2M1 times a power of two is exact in BF16), and stored to tensor memory, from which the MMA
-// reads A without passing through shared memory, whose bandwidth 32 KB per K block in and out
-// would fill. Products and activations are exact, sums are FP32.
+// The weight is the A operand of tcgen05 MMAs (128 weight rows are the 128 lanes of tensor
+// memory, up to 64 activation rows the N columns): every code is expanded once, in registers, to
+// the BF16 value it stands for (E2M1 times a power of two is exact in BF16), and stored to
+// tensor memory, from which the MMA reads A without passing through shared memory, whose
+// bandwidth 32 KB per K block in and out would fill. Products are exact, sums are FP32.
 //
-// A CTA takes 128 weight rows (SwiGLU: 64 gate rows and their 64 up rows) and a slice of K. TMA
-// brings code tiles, x tiles and scale tiles through a ring; eight warps expand; one thread
-// issues the MMAs. A cluster of up to eight CTAs shares the K blocks of one row tile, so that
-// weights of few rows still occupy the GPU; their FP32 partial sums are added through
-// distributed shared memory in rank order (deterministic).
+// A CTA takes 128 weight rows (SwiGLU: 64 gate rows and their 64 up rows) and a slice of K. Four
+// warps copy codes and scales asynchronously into a ring, TMA brings x tiles beside them,
+// eight warps expand, one thread issues the MMAs. (Codes by TMA come in boxes of 64-byte rows,
+// whose requests alone took 33 us at n = 28672, k = 8192.) A cluster of up to eight CTAs shares
+// the K blocks of one row tile, so that weights of few rows still occupy the GPU; their FP32
+// partial sums are added through distributed shared memory in rank order (deterministic).
+//
+// Bound: 64 rows, n = 28672, k = 8192 takes 61 us (125 MB of weight, 2.1 TB/s, 0.49 PFLOP/s): a K
+// block costs an SM 0.3 us of expansion, MMA and hand-over, where its bytes take 0.2. Small
+// weights pay the chain through one CTA, about 6 us (64 rows, n = 1024, k = 4096: 8.1 us).
 #include <algorithm>
 
 #include "internal.h"
@@ -30,17 +31,18 @@ namespace {
 constexpr int kM = 128;            // weight rows per CTA
 constexpr int kKB = 128;           // K elements per ring stage
 constexpr int kExpandWarps = 8;
-constexpr int kThreads = 64 + 32 * kExpandWarps;
+constexpr int kCopyThreads = 128;
+constexpr int kThreads = 64 + 32 * kExpandWarps + kCopyThreads;
 constexpr int kABuffers = 3;       // expanded K blocks in tensor memory, 64 columns each
 constexpr int kACol = 64;          // first column of the A buffers (D before it)
 constexpr uint32_t kTmemCols = 256;
 constexpr int kMaxSplit = 8;
 
-template <int R, bool SWIGLU>
+template <int R>
 struct ProductSmem {
   static constexpr int kCodeBytes = kM * kKB / 2;
   static constexpr int kXBytes = R * kKB * 2;
-  static constexpr int kSfBytes = SWIGLU ? 2048 : 1024;  // 3 or 1 scale tiles of 512 bytes
+  static constexpr int kSfBytes = 1024;  // four scale bytes a row
   static constexpr int kStageBytes = kCodeBytes + kXBytes + kSfBytes;
   // Two CTAs per SM: while one drains its pipeline the other streams.
   static constexpr int kStages = (113 * 1024 - 2048) / kStageBytes;
@@ -53,30 +55,38 @@ struct ProductSmem {
 };
 
 // The 32 codes of one group (16 bytes) as 16 registers of two BF16 values each.
-__device__ __forceinline__ void expand_group(const uint4& q, uint32_t scale, uint32_t* out) {
-  const uint32_t f = mx4_factor(scale);
+template <bool WIDE>
+__device__ __forceinline__ void expand_group(const uint4& q, uint32_t scale, const Mx4Spread& m, uint32_t* out) {
+  const uint32_t f = WIDE ? mx4_wide_factor(scale) : mx4_factor(scale);
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint32_t v[4];
-    mx4_expand(w[i], f, v);
+    mx4_expand(w[i], f, m, v);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) out[4 * i + j] = v[j];
+    for (int j = 0; j < 4; ++j) out[4 * i + j] = WIDE ? mul_bf16x2(v[j], mx4_factor2(scale)) : v[j];
   }
-  if (__any_sync(0xffffffffu, scale > 128u)) {
-    const uint32_t g = mx4_factor2(scale);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) out[i] = mul_bf16x2(out[i], g);
-  }
+}
+
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+__device__ __forceinline__ void copy_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// Arrives on the barrier once this thread's copies so far have landed.
+__device__ __forceinline__ void copy_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 template <int R, bool SWIGLU>
 __global__ void __launch_bounds__(kThreads, 2)
-    mx4_product_kernel(const __grid_constant__ CUtensorMap tm_codes,
-                       const __grid_constant__ CUtensorMap tm_x, const uint8_t* scales,
-                       const bf16* residual, bf16* out, int rows, int n, int kblocks, int split,
+    mx4_product_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* codes,
+                       const uint8_t* scales, const bf16* residual, bf16* out, int rows, int n, int kblocks, int split,
                        int* err) {
-  using L = ProductSmem<R, SWIGLU>;
+  using L = ProductSmem<R>;
   constexpr int NS = L::kStages;
   constexpr int kCols = SWIGLU ? 64 : 128;  // output columns per CTA
 
@@ -99,13 +109,15 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int tile = static_cast<int>(blockIdx.x) / split;
   const int row0 = static_cast<int>(blockIdx.y) * R;
   const int kb0 = kblocks * rank / split, kb1 = kblocks * (rank + 1) / split;
-  // First weight rows of the tile (SwiGLU: of its gate half and of its up half).
   const int w0 = tile * kCols;
-  const int up0 = n + w0;
+  // Weight row of tile row r; rows past the last one (of its half) read it again, unused.
+  auto weight_row = [&](int r) {
+    return SWIGLU ? min(w0 + r % 64, n - 1) + (r / 64) * n : min(w0 + r, n - 1);
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
-      mbar_init(full_bar(s), 1);
+      mbar_init(full_bar(s), 1 + kCopyThreads);
       mbar_init(empty_bar(s), 1);
     }
     for (int a = 0; a < kABuffers; ++a) {
@@ -129,12 +141,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (warp == 0) {
     if (lane == 0) {
-      tma_prefetch_desc(&tm_codes);
       tma_prefetch_desc(&tm_x);
-      // Scale tiles of the rows: one, or the gate rows' and the up rows' (which may straddle two).
-      const int tiles = ((SWIGLU ? 2 * n : n) + 127) / 128;
-      const int t0 = w0 / 128, t1 = up0 / 128, t2 = min(t1 + 1, tiles - 1);
-      const uint32_t bytes = L::kCodeBytes + L::kXBytes + (SWIGLU ? 1536u : 512u);
       int it = 0;
       bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb, ++it) {
@@ -144,23 +151,10 @@ __global__ void __launch_bounds__(kThreads, 2)
           ok = false;
           break;
         }
-        const uint32_t codes = base + s * L::kStageBytes;
-        const uint32_t xs = codes + L::kCodeBytes;
-        const uint32_t sf = xs + L::kXBytes;
-        mbar_arrive_expect_tx(full_bar(s), bytes);
-        if constexpr (SWIGLU) {
-          tma_load_2d(codes, &tm_codes, full_bar(s), kb * 64, w0);
-          tma_load_2d(codes + L::kCodeBytes / 2, &tm_codes, full_bar(s), kb * 64, up0);
-        } else {
-          tma_load_2d(codes, &tm_codes, full_bar(s), kb * 64, w0);
-        }
+        const uint32_t xs = base + s * L::kStageBytes + L::kCodeBytes;
+        mbar_arrive_expect_tx(full_bar(s), L::kXBytes);
         tma_load_2d(xs, &tm_x, full_bar(s), kb * kKB, row0);
         tma_load_2d(xs + L::kXBytes / 2, &tm_x, full_bar(s), kb * kKB + 64, row0);
-        bulk_load(sf, scales + (static_cast<size_t>(t0) * kblocks + kb) * 512, 512, full_bar(s));
-        if constexpr (SWIGLU) {
-          bulk_load(sf + 512, scales + (static_cast<size_t>(t1) * kblocks + kb) * 512, 512, full_bar(s));
-          bulk_load(sf + 1024, scales + (static_cast<size_t>(t2) * kblocks + kb) * 512, 512, full_bar(s));
-        }
       }
       if (!ok) {  // the copies in flight land before the CTA may end
         for (int i = max(0, it - NS); i < it; ++i) mbar_wait(full_bar(i % NS), (i / NS) & 1);
@@ -192,20 +186,37 @@ __global__ void __launch_bounds__(kThreads, 2)
       umma_commit(done_bar);
     }
     __syncwarp();
+  } else if (warp >= 2 + kExpandWarps) {
+    const int ct = threadIdx.x - 64 - 32 * kExpandWarps;
+    const uint8_t* src[4];  // 16 bytes (a scale group) of rows ct / 4 + 32 i
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      src[i] = codes + (static_cast<size_t>(weight_row(i * 32 + ct / 4)) * kblocks + kb0) * 64 + ct % 4 * 16;
+    }
+    const uint32_t dst = (ct / 4) * 64 + (((ct % 4) ^ (ct / 8 & 3)) << 4);
+    const int sr = weight_row(ct);
+    const uint8_t* scale_src = scales + (static_cast<size_t>(sr / 128) * kblocks + kb0) * 512 + (sr % 32) * 16 + (sr / 32 % 4) * 4;
+    for (int it = 0; it < kb1 - kb0; ++it) {
+      const int s = it % NS;
+      if (!mbar_wait(empty_bar(s), ((it / NS) & 1) ^ 1)) {
+        record_error(err, kErrTimeoutProducer);
+        break;
+      }
+      const uint32_t stage = base + s * L::kStageBytes;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) copy_async16(stage + dst + i * 32 * 64, src[i] + it * 64);
+      copy_async4(stage + L::kCodeBytes + L::kXBytes + ct * 4, scale_src + static_cast<size_t>(it) * 512);
+      copy_arrive(full_bar(s));
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
     // Four warps cover the 128 lanes; the first four expand the even stages, the others the odd.
     const int turn = (warp - 2) / 4;
     const int r = (warp & 3) * 32 + lane;           // weight row in the tile = lane of TMEM
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    // Where the row's four scale bytes of a K block lie in the stage's scale tiles.
-    int tile_row = r, area = 0;
-    if constexpr (SWIGLU) {
-      const int wrow = r < 64 ? w0 + r : up0 + r - 64;
-      tile_row = wrow % 128;
-      area = r < 64 ? 0 : 1 + (wrow / 128 - up0 / 128);
-    }
-    const uint32_t sf_off = L::kCodeBytes + L::kXBytes + area * 512 + (tile_row % 32) * 16 + (tile_row / 32) * 4;
+    const uint32_t sf_off = L::kCodeBytes + L::kXBytes + r * 4;
     const uint32_t swz = (r >> 1) & 3;
+    const Mx4Spread spread;
     for (int it = turn; it < kb1 - kb0; it += 2) {
       const int s = it % NS, a = it % kABuffers;
       if (!mbar_wait(full_bar(s), (it / NS) & 1)) {
@@ -230,9 +241,15 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (uint32_t h = 0; h < 2; ++h) {
         const uint4 q0 = ld_shared_v4(row + (((2u * h) ^ swz) << 4));
         const uint4 q1 = ld_shared_v4(row + (((2u * h + 1u) ^ swz) << 4));
+        const uint32_t s0 = (sf >> (16u * h)) & 255u, s1 = (sf >> (16u * h + 8u)) & 255u;
         uint32_t v[32];
-        expand_group(q0, (sf >> (16u * h)) & 255u, v);
-        expand_group(q1, (sf >> (16u * h + 8u)) & 255u, v + 16);
+        if (__any_sync(0xffffffffu, max(s0, s1) > 128u)) {
+          expand_group<true>(q0, s0, spread, v);
+          expand_group<true>(q1, s1, spread, v + 16);
+        } else {
+          expand_group<false>(q0, s0, spread, v);
+          expand_group<false>(q1, s1, spread, v + 16);
+        }
         tmem_st32(tmem + lane_base + kACol + 64u * a + 32u * h, v);
       }
       tmem_st_wait();
@@ -294,36 +311,26 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (split > 1) cluster_sync_all();  // a peer may still read this CTA's sums
 }
 
-// CTAs per row tile. The CTAs of an SM share its issue slots, so a launch takes as long as the
-// SM with the most of them: ceil(tiles * split / SMs) times kblocks / split ring stages and a
-// fixed part (launch, tensor memory, pipeline fill, join) worth about kFixed stages.
+// CTAs per row tile: as many as fit on the GPU at once (two an SM), with at least four K blocks
+// each. A CTA costs about 6 us beside its blocks (tensor memory, first bytes, join), 0.3 to 0.4
+// us each, so that a second wave never pays: 33 rows, n = 8192 (SwiGLU), k = 2048 takes 13.9 us
+// unsplit, 12.9 at 2 and 19.4 at 3, the first split of more CTAs than fit.
 int choose_split(int tiles, int kblocks) {
-  constexpr int kFixed = 3;
-  const int sms = sm_count();
-  int best = 1;
-  int64_t best_cost = INT64_MAX;
-  for (int split = 1; split <= std::min(kMaxSplit, kblocks); ++split) {
-    const int64_t turns = (static_cast<int64_t>(tiles) * split + sms - 1) / sms;
-    const int64_t cost = turns * ((kblocks + split - 1) / split + kFixed);
-    if (cost < best_cost) best_cost = cost, best = split;
-  }
-  return best;
+  return std::max(1, std::min({kMaxSplit, 2 * sm_count() / tiles, kblocks / 4}));
 }
 
 template <int R, bool SWIGLU>
 void launch_product(const bf16* x, const uint8_t* codes, const uint8_t* scales,
                     const bf16* residual, bf16* out, int rows, int n, int k, cudaStream_t s) {
-  using L = ProductSmem<R, SWIGLU>;
+  using L = ProductSmem<R>;
   auto kernel = mx4_product_kernel<R, SWIGLU>;
   ensure_smem(kernel, L::kBytes);
   constexpr int kCols = SWIGLU ? 64 : 128;
-  const int wide = SWIGLU ? 2 * n : n;
-  const CUtensorMap tc = make_tmap_u8_sw64(codes, wide, k / 2, k / 2, kCols);
   const CUtensorMap tx = make_tmap_bf16(x, rows, k, k, R);
   const int tiles = (n + kCols - 1) / kCols, kblocks = k / kKB;
   const int split = choose_split(tiles * ((rows + R - 1) / R), kblocks);
   const dim3 grid(static_cast<unsigned>(tiles * split), static_cast<unsigned>((rows + R - 1) / R));
-  launch(kernel, grid, kThreads, L::kBytes, split > 1 ? split : 0, s, tc, tx, scales, residual, out,
+  launch(kernel, grid, kThreads, L::kBytes, split > 1 ? split : 0, s, tx, codes, scales, residual, out,
          rows, n, kblocks, split, device_error_word());
 }
 
@@ -332,16 +339,15 @@ void launch_product(const bf16* x, const uint8_t* codes, const uint8_t* scales,
 void mx4_product_tc(const bf16* x, const uint8_t* codes, const uint8_t* scales,
                     const bf16* residual, bf16* out, int rows, int n, int k, bool swiglu,
                     cudaStream_t s) {
-  if (swiglu) {
-    if (rows <= 32) {
-      launch_product<32, true>(x, codes, scales, nullptr, out, rows, n, k, s);
-    } else {
-      launch_product<64, true>(x, codes, scales, nullptr, out, rows, n, k, s);
-    }
-  } else if (rows <= 32) {
-    launch_product<32, false>(x, codes, scales, residual, out, rows, n, k, s);
+  auto run = [&](auto product, auto swiglu_product) {
+    (swiglu ? swiglu_product : product)(x, codes, scales, residual, out, rows, n, k, s);
+  };
+  if (rows <= 32) {
+    run(launch_product<32, false>, launch_product<32, true>);
+  } else if (rows <= 48) {
+    run(launch_product<48, false>, launch_product<48, true>);
   } else {
-    launch_product<64, false>(x, codes, scales, residual, out, rows, n, k, s);
+    run(launch_product<64, false>, launch_product<64, true>);
   }
 }
 

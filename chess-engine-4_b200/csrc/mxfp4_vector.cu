@@ -1,15 +1,22 @@
-// Products of very few BF16 activation rows with an MXFP4 weight (kernel-op API mxfp4_linear,
+// Products of up to 32 BF16 activation rows with an MXFP4 weight (kernel-op API mxfp4_linear,
 // mxfp4_swiglu), and the choice between this form and the tcgen05 one.
 //
 // The time is the weight's 0.53 bytes per element as long as a code costs at most three
 // lane operations (an SM takes in about 43 codes a clock at the memory's rate and issues 128
-// lane operations), of which expanding it to BF16 takes 2.1 (mxfp4.cuh). With up to 32 rows the
-// rest is a warp-level MMA per 8 codes a lane and 8 rows, whose A fragment is made in the very
-// registers that the codes were loaded into: no shared memory, no barrier and no hand-over
-// between warps until the sums are joined, so that any number of warps hides the memory's
-// latency. A warp takes 16 weight rows (SwiGLU: 8 gate rows and their 8 up rows, which meet in
-// one thread) and every eighth K block of 128 columns; a lane's 16 bytes of a row are one scale
-// group. The eight warps' sums are added in shared memory in a fixed order (deterministic).
+// lane operations), of which expanding it to BF16 takes 2.1 (mxfp4.cuh). The rest is a
+// warp-level MMA per 8 codes a lane and 8 rows, whose A fragment is made in the very registers
+// that the codes were loaded into: no shared memory, no barrier and no hand-over between warps
+// until the sums are joined, so that any number of warps hides the memory's latency. A warp
+// takes one or two tiles of 16 weight rows (SwiGLU: 8 gate rows and their 8 up rows, which meet
+// in one thread) and every eighth K block of 128 columns; a lane's 16 bytes of a row are one
+// scale group. The eight warps' sums are added in shared memory in a fixed order
+// (deterministic).
+//
+// 1 row, n = 512, k = 1536: 2.2 us, of which the launch is 1.5. 7 rows, n = 28672, k = 8192:
+// 39.7 us (125 MB of weight, 3.2 TB/s), bound by the instructions of the expansion and by x's
+// 64-byte pieces in the load pipeline. (x resident in shared memory with one CTA of 16 warps per
+// SM and codes by asynchronous copies: 44 us; the tensor core's own E2M1 operand, which needs x
+// in 8-bit terms made by a second kernel: 50 us.)
 #include <algorithm>
 
 #include "internal.h"
@@ -31,20 +38,50 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Weight bytes are read once: they leave the L1 cache to x.
-__device__ __forceinline__ uint4 load_stream(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
+// The 64 codes a lane has of a K block (fragment rows g and g + 8 of the tile) times x's
+// fragments, which fragment(j, i) gives for n-tile j and word i.
+template <int NT, bool WIDE, class Fragment>
+__device__ __forceinline__ void multiply_block(const uint4 (&q)[2], const uint32_t (&scale)[2], const Mx4Spread& spread,
+                                               Fragment fragment, float (&acc)[NT][4]) {
+  uint32_t f[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) f[h] = WIDE ? mx4_wide_factor(scale[h]) : mx4_factor(scale[h]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t a[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      mx4_expand(i == 0 ? q[h].x : i == 1 ? q[h].y : i == 2 ? q[h].z : q[h].w, f[h], spread, a[h]);
+      if constexpr (WIDE) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[h][e] = mul_bf16x2(a[h][e], mx4_factor2(scale[h]));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const uint4 b = fragment(j, i);
+      mma_bf16(acc[j], a[0][0], a[1][0], a[0][1], a[1][1], b.x, b.y);
+      mma_bf16(acc[j], a[0][2], a[1][2], a[0][3], a[1][3], b.z, b.w);
+    }
+  }
+}
+
+template <int NT, class Fragment>
+__device__ __forceinline__ void multiply_block(const uint4 (&q)[2], const uint32_t (&scale)[2], const Mx4Spread& spread,
+                                               Fragment fragment, float (&acc)[NT][4]) {
+  if (__any_sync(0xffffffffu, max(scale[0], scale[1]) > 128u)) {
+    multiply_block<NT, true>(q, scale, spread, fragment, acc);
+  } else {
+    multiply_block<NT, false>(q, scale, spread, fragment, acc);
+  }
 }
 
 template <int NT, int MT, bool SWIGLU>
-__global__ void __launch_bounds__(32 * kWarps)
+__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : NT == 2 ? 2 : 1)
     mx4_vector_kernel(const bf16* x, const uint8_t* codes, const uint8_t* scales,
                       const bf16* residual, bf16* out, int rows, int n, int k) {
-  constexpr int kCols = (SWIGLU ? 8 : 16) * MT;  // output columns per CTA
+  constexpr int kTileCols = SWIGLU ? 8 : 16;
+  constexpr int kCols = MT * kTileCols;  // output columns per CTA
   __shared__ float part[kWarps][8 * NT][16 * MT + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -53,14 +90,15 @@ __global__ void __launch_bounds__(32 * kWarps)
   grid_dependency_wait();
   grid_launch_dependents();
 
-  // Fragment row h of tile m: weight rows past the last one read it again, unused.
+  // Weight rows past the last one read it again, unused.
   const uint8_t* code_ptr[MT][2];
   const uint8_t* scale_ptr[MT][2];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int wrow = SWIGLU ? min(col0 + 8 * m + g, n - 1) + h * n : min(col0 + 16 * m + 8 * h + g, n - 1);
+      const int col = col0 + m * kTileCols + g;
+      const int wrow = SWIGLU ? min(col, n - 1) + h * n : min(col + 8 * h, n - 1);
       code_ptr[m][h] = codes + static_cast<size_t>(wrow) * (k / 2) + t * 16;
       scale_ptr[m][h] = scales + static_cast<size_t>(wrow / 128) * kblocks * 512 + (wrow % 32) * 16 +
                         (wrow / 32 % 4) * 4 + t;
@@ -72,68 +110,38 @@ __global__ void __launch_bounds__(32 * kWarps)
     x_ptr[j] = row0 + 8 * j + g < rows ? x + static_cast<size_t>(row0 + 8 * j + g) * k + t * 32 : nullptr;
   }
 
+  const Mx4Spread spread;
   float acc[MT][NT][4] = {};
-  uint4 q[MT][2];
-  uint32_t sc[MT][2];
-  auto load = [&](int kb) {
+  uint4 next[2];
+  uint32_t next_scale[2];
+  auto load = [&](int m, int kb) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        q[m][h] = load_stream(code_ptr[m][h] + kb * 64);
-        sc[m][h] = scale_ptr[m][h][static_cast<size_t>(kb) * 512];
-      }
+    for (int h = 0; h < 2; ++h) {
+      next[h] = load_stream(code_ptr[m][h] + kb * 64);
+      next_scale[h] = scale_ptr[m][h][static_cast<size_t>(kb) * 512];
     }
   };
-  int kb = warp;
-  if (kb < kblocks) load(kb);
-  while (kb < kblocks) {
+  if (warp < kblocks) load(0, warp);
+  for (int kb = warp; kb < kblocks; kb += kWarps) {
     uint4 xv[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        xv[j][i] = x_ptr[j] != nullptr ? *reinterpret_cast<const uint4*>(x_ptr[j] + static_cast<size_t>(kb) * 128 + i * 8)
+        xv[j][i] = x_ptr[j] != nullptr ? permute_x(*reinterpret_cast<const uint4*>(x_ptr[j] + static_cast<size_t>(kb) * 128 + i * 8))
                                        : make_uint4(0u, 0u, 0u, 0u);
       }
     }
-    uint4 c[MT][2];
-    uint32_t s[MT][2], f[MT][2], top = 0;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        c[m][h] = q[m][h];
-        s[m][h] = sc[m][h];
-        f[m][h] = mx4_factor(s[m][h]);
-        top = max(top, s[m][h]);
+      const uint4 q[2] = {next[0], next[1]};
+      const uint32_t scale[2] = {next_scale[0], next_scale[1]};
+      if (m + 1 < MT) {
+        load(m + 1, kb);
+      } else if (kb + kWarps < kblocks) {
+        load(0, kb + kWarps);
       }
-    }
-    kb += kWarps;
-    if (kb < kblocks) load(kb);
-    const bool wide = __any_sync(0xffffffffu, top > 128u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint4 b[NT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) b[j] = permute_x(xv[j][i]);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        uint32_t a[2][4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          mx4_expand(i == 0 ? c[m][h].x : i == 1 ? c[m][h].y : i == 2 ? c[m][h].z : c[m][h].w, f[m][h], a[h]);
-          if (wide) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) a[h][e] = mul_bf16x2(a[h][e], mx4_factor2(s[m][h]));
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          mma_bf16(acc[m][j], a[0][0], a[1][0], a[0][1], a[1][1], b[j].x, b[j].y);
-          mma_bf16(acc[m][j], a[0][2], a[1][2], a[0][3], a[1][3], b[j].z, b[j].w);
-        }
-      }
+      multiply_block<NT>(q, scale, spread, [&](int j, int i) { return xv[j][i]; }, acc[m]);
     }
   }
   // A lane holds weight rows g and g + 8, activation rows 2t and 2t + 1 of each 8.
@@ -171,20 +179,37 @@ void launch_vector(const bf16* x, const uint8_t* codes, const uint8_t* scales, c
   launch(mx4_vector_kernel<NT, MT, SWIGLU>, grid, 32 * kWarps, 0, 0, s, x, codes, scales, residual, out, rows, n, k);
 }
 
-#ifndef VMT
-#define VMT 1
-#endif
+// Two row tiles a warp read x once for both, which counts as soon as CTAs are many; one tile a
+// warp spreads a small weight over more SMs. Measured (us, one tile | two): 7 rows 4096 x 4096
+// 6.2 | 7.2, 28672 x 8192 45.2 | 39.7; 16 rows 1024 x 4096 6.6 | 6.9, 4096 x 4096 9.1 | 7.6,
+// 28672 x 8192 79.6 | 55.4.
+template <int NT, bool SWIGLU>
+void choose_tiles(const bf16* x, const uint8_t* codes, const uint8_t* scales, const bf16* residual,
+                  bf16* out, int rows, int n, int k, cudaStream_t s) {
+  const int tiles = (n + (SWIGLU ? 7 : 15)) / (SWIGLU ? 8 : 16);
+  if (tiles >= (NT == 1 ? 4 : 1) * sm_count()) {
+    launch_vector<NT, 2, SWIGLU>(x, codes, scales, residual, out, rows, n, k, s);
+  } else {
+    launch_vector<NT, 1, SWIGLU>(x, codes, scales, residual, out, rows, n, k, s);
+  }
+}
+
+// Up to 16 rows this form is the faster one at every size. With 17 to 32 rows the MMAs and x's
+// fragments weigh more than the codes, and the tcgen05 form wins once its fixed 5 us are
+// spread over enough codes: 32 rows, codes in millions, this form | tcgen05 (us): 0.8 4.5 | 5.1,
+// 1.6 3.4 | 4.7, 4.2 8.5 | 6.6, 16.8 10.4 | 9.6, 235 100 | 63.
 template <bool SWIGLU>
 void product(const bf16* x, const uint8_t* codes, const uint8_t* scales, const bf16* residual,
              bf16* out, int rows, int n, int k, cudaStream_t s) {
-  if (rows <= 8) {
-    launch_vector<1, VMT, SWIGLU>(x, codes, scales, residual, out, rows, n, k, s);
-  } else if (rows <= 16) {
-    launch_vector<2, VMT, SWIGLU>(x, codes, scales, residual, out, rows, n, k, s);
-  } else if (rows <= 32) {
-    launch_vector<4, VMT, SWIGLU>(x, codes, scales, residual, out, rows, n, k, s);
-  } else {
+  const int64_t weight = static_cast<int64_t>(n) * k * (SWIGLU ? 2 : 1);
+  if (rows > 32 || (rows > 16 && weight > (1 << 21))) {
     mx4_product_tc(x, codes, scales, residual, out, rows, n, k, SWIGLU, s);
+  } else if (rows <= 8) {
+    choose_tiles<1, SWIGLU>(x, codes, scales, residual, out, rows, n, k, s);
+  } else if (rows <= 16) {
+    choose_tiles<2, SWIGLU>(x, codes, scales, residual, out, rows, n, k, s);
+  } else {
+    choose_tiles<4, SWIGLU>(x, codes, scales, residual, out, rows, n, k, s);
   }
 }
 

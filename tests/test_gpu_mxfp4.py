@@ -120,7 +120,7 @@ def test_linear_over_row_counts(rows: int) -> None:
     _assert_product(kernels.mxfp4_linear(x, q, residual=residual), ref + residual.cpu().double(), mags, k)
 
 
-@pytest.mark.parametrize("rows", [1, 12, 64])
+@pytest.mark.parametrize("rows", [1, 12, 20, 48, 64])
 @pytest.mark.parametrize("n,k", SHAPES)
 def test_linear_over_shapes(rows: int, n: int, k: int) -> None:
     from ce4b200 import kernels
@@ -136,8 +136,23 @@ def test_linear_over_shapes(rows: int, n: int, k: int) -> None:
     _assert_product(kernels.mxfp4_linear(x, q), ref, mags, k)
 
 
-@pytest.mark.parametrize("rows", [1, 5, 17, 33, 64, 100])
-@pytest.mark.parametrize("hidden,k", [(1, 128), (64, 256), (100, 128), (192, 512), (1536, 512), (300, 2048)])
+@pytest.mark.parametrize("n,k", [(2400, 256), (9500, 384), (20001, 128), (1030, 8192), (4100, 1152)])
+@pytest.mark.parametrize("rows", [3, 9, 30, 41])
+def test_linear_over_large_weights(rows: int, n: int, k: int) -> None:
+    """Weights of many row tiles, or of K blocks that the warps share unevenly."""
+
+    from ce4b200 import kernels
+
+    g = torch.Generator().manual_seed(n)
+    q = kernels.quantize_mxfp4(_weight(n, k, 5, spread=2).cuda())
+    x = torch.randn(rows, k, generator=g).bfloat16().cuda()
+    residual = torch.randn(rows, n, generator=g).bfloat16().cuda()
+    ref, mags = _product(x, _values(q))
+    _assert_product(kernels.mxfp4_linear(x, q, residual=residual), ref + residual.cpu().double(), mags, k)
+
+
+@pytest.mark.parametrize("rows", [1, 5, 12, 17, 33, 64, 100])
+@pytest.mark.parametrize("hidden,k", [(1, 128), (64, 256), (100, 128), (192, 512), (1536, 512), (300, 2048), (4777, 256)])
 def test_swiglu(rows: int, hidden: int, k: int) -> None:
     """silu(g) u is off by |d(silu u)| <= 1.1 |u| dg + |silu(g)| du for sums off by dg, du
     (|silu'| < 1.1), by a few FP32 roundings of the formula, and by one BF16 rounding."""
