@@ -616,6 +616,7 @@ int ce4b_add_rmsnorm_mxfp8(const void* x_dev, const void* residual_dev, const vo
     require(x_dev && weight_dev && codes_dev && scales_dev, "null pointer");
     require(residual_dev == nullptr || sum_dev != nullptr, "a residual needs an output for the sum");
     require(rows >= 1 && width >= 1, "extents must be positive");
+    require(rows <= INT32_MAX - 127, "too many rows");
     require(width % 128 == 0, "MXFP8 rows need a width that is a multiple of 128");
     require(aligned(codes_dev, 16), "MXFP8 codes must be 16-byte aligned");
     add_rmsnorm_rows(static_cast<const bf16*>(x_dev), static_cast<const bf16*>(residual_dev),

@@ -129,9 +129,6 @@ void mx_quantize_transpose(const bf16* x, uint8_t* codes, uint8_t* scales, int r
 // 2-D byte (E4M3 code) tensor map, 128-byte swizzle, box = 128 codes x box_rows.
 CUtensorMap make_tmap_u8(const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld_bytes,
                          uint32_t box_rows);
-// Same with a 64-byte swizzle and box = 64 bytes x box_rows.
-CUtensorMap make_tmap_u8_sw64(const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld_bytes,
-                              uint32_t box_rows);
 // C[M,N] BF16 = block-scaled E4M3 A[M,K] . B[N,K]^T (N, K multiples of 128, A's scale
 // tiles padded to 128 rows; maps with
 // 128-row boxes; C map BF16 with 128-row boxes).

@@ -315,8 +315,9 @@ __global__ void __launch_bounds__(kThreads, 2)
 // each. A CTA costs about 6 us beside its blocks (tensor memory, first bytes, join), 0.3 to 0.4
 // us each, so that a second wave never pays: 33 rows, n = 8192 (SwiGLU), k = 2048 takes 13.9 us
 // unsplit, 12.9 at 2 and 19.4 at 3, the first split of more CTAs than fit.
-int choose_split(int tiles, int kblocks) {
-  return std::max(1, std::min({kMaxSplit, 2 * sm_count() / tiles, kblocks / 4}));
+int choose_split(int64_t tiles, int kblocks) {
+  const int fit = static_cast<int>(2 * sm_count() / tiles);
+  return std::max(1, std::min({kMaxSplit, fit, kblocks / 4}));
 }
 
 template <int R, bool SWIGLU>
@@ -327,9 +328,10 @@ void launch_product(const bf16* x, const uint8_t* codes, const uint8_t* scales,
   ensure_smem(kernel, L::kBytes);
   constexpr int kCols = SWIGLU ? 64 : 128;
   const CUtensorMap tx = make_tmap_bf16(x, rows, k, k, R);
-  const int tiles = (n + kCols - 1) / kCols, kblocks = k / kKB;
-  const int split = choose_split(tiles * ((rows + R - 1) / R), kblocks);
-  const dim3 grid(static_cast<unsigned>(tiles * split), static_cast<unsigned>((rows + R - 1) / R));
+  const int tiles = (n - 1) / kCols + 1, blocks = (rows - 1) / R + 1, kblocks = k / kKB;
+  require(blocks <= 65535, "MXFP4 products take at most 65535 blocks of 64 rows");
+  const int split = choose_split(static_cast<int64_t>(tiles) * blocks, kblocks);
+  const dim3 grid(static_cast<unsigned>(tiles) * split, static_cast<unsigned>(blocks));
   launch(kernel, grid, kThreads, L::kBytes, split > 1 ? split : 0, s, tx, codes, scales, residual, out,
          rows, n, kblocks, split, device_error_word());
 }

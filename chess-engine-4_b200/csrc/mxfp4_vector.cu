@@ -175,7 +175,7 @@ template <int NT, int MT, bool SWIGLU>
 void launch_vector(const bf16* x, const uint8_t* codes, const uint8_t* scales, const bf16* residual,
                    bf16* out, int rows, int n, int k, cudaStream_t s) {
   constexpr int kCols = (SWIGLU ? 8 : 16) * MT;
-  const dim3 grid(static_cast<unsigned>((n + kCols - 1) / kCols), static_cast<unsigned>((rows + 8 * NT - 1) / (8 * NT)));
+  const dim3 grid(static_cast<unsigned>((n - 1) / kCols + 1), static_cast<unsigned>((rows - 1) / (8 * NT) + 1));
   launch(mx4_vector_kernel<NT, MT, SWIGLU>, grid, 32 * kWarps, 0, 0, s, x, codes, scales, residual, out, rows, n, k);
 }
 
@@ -186,7 +186,7 @@ void launch_vector(const bf16* x, const uint8_t* codes, const uint8_t* scales, c
 template <int NT, bool SWIGLU>
 void choose_tiles(const bf16* x, const uint8_t* codes, const uint8_t* scales, const bf16* residual,
                   bf16* out, int rows, int n, int k, cudaStream_t s) {
-  const int tiles = (n + (SWIGLU ? 7 : 15)) / (SWIGLU ? 8 : 16);
+  const int tiles = (n - 1) / (SWIGLU ? 8 : 16) + 1;
   if (tiles >= (NT == 1 ? 4 : 1) * sm_count()) {
     launch_vector<NT, 2, SWIGLU>(x, codes, scales, residual, out, rows, n, k, s);
   } else {

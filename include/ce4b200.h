@@ -467,8 +467,9 @@ int ce4b_dequantize_mxfp4(const void* codes_dev, const void* scales_dev, void* o
 
 /* out[rows, n] = bf16(x[rows, k] . W[n, k]^T + residual[rows, n]) with an MXFP4 weight
  * (FP32 sums, rounded once); residual_dev may be NULL, and may be out_dev itself. For few
- * rows (search batches): the time goes to reading the 4-bit weight once per 64 rows. x, codes and scales
- * are 16-byte aligned, k is a multiple of 128. A row of x that holds a NaN or an infinity
+ * rows (search batches): the time goes to reading the 4-bit weight, once per 64 rows (at most
+ * 65535 times). x, codes and scales are 16-byte aligned, k is a multiple of 128. Weights count
+ * with the values ce4b_dequantize_mxfp4 gives. A row of x that holds a NaN or an infinity
  * gives a row of non-finite values. */
 int ce4b_mxfp4_linear(const void* x_dev, const void* codes_dev, const void* scales_dev,
                       const void* residual_dev, void* out_dev, int rows, int n, int k,

@@ -198,6 +198,24 @@ def test_scales_over_the_whole_range(power: int) -> None:
     _assert_product(kernels.mxfp4_linear(x, q), ref, mags, 256)
 
 
+@pytest.mark.parametrize("rows", [2, 40])
+@pytest.mark.parametrize("low", [0, 1, 5, 40, 200, 245])
+def test_scale_codes_of_other_quantisers(rows: int, low: int) -> None:
+    """Scales that quantize_mxfp4 does not choose: from 2^-127 (weights that are subnormal in
+    BF16) to 2^121."""
+
+    from ce4b200 import kernels
+
+    g = torch.Generator().manual_seed(low)
+    codes = torch.randint(0, 256, (140, 128), generator=g, dtype=torch.uint8)
+    scales = torch.randint(low, low + 4, (2, 2, 32, 16), generator=g, dtype=torch.uint8)
+    q = kernels.Mxfp4Tensor(codes.cuda(), scales.cuda())
+    assert torch.equal(kernels.dequantize_mxfp4(q).cpu().double(), _values(q))
+    x = (torch.randn(rows, 256, generator=g) * 2.0 ** max(-100, min(110, 127 - low))).bfloat16().cuda()
+    ref, mags = _product(x, _values(q))
+    _assert_product(kernels.mxfp4_linear(x, q), ref, mags, 256)
+
+
 def test_tiny_and_huge_activations() -> None:
     from ce4b200 import kernels
 
@@ -210,24 +228,25 @@ def test_tiny_and_huge_activations() -> None:
         _assert_product(kernels.mxfp4_linear(x, q), ref, mags, 256)
 
 
-def test_values_that_are_not_finite_stay_in_their_row() -> None:
+@pytest.mark.parametrize("rows", [12, 20, 40])
+def test_values_that_are_not_finite_stay_in_their_row(rows: int) -> None:
     from ce4b200 import kernels
 
     g = torch.Generator().manual_seed(3)
     w = _weight(300, 512, 12)
     q = kernels.quantize_mxfp4(w.cuda())
-    x = torch.randn(20, 512, generator=g).bfloat16()
+    x = torch.randn(rows, 512, generator=g).bfloat16()
     clean = kernels.mxfp4_linear(x.cuda(), q)
     x[3, 100] = float("nan")
     x[11, 511] = float("inf")
     got = kernels.mxfp4_linear(x.cuda(), q)
-    rows = [r for r in range(20) if r not in (3, 11)]
-    assert torch.equal(got[rows], clean[rows])
+    others = [r for r in range(rows) if r not in (3, 11)]
+    assert torch.equal(got[others], clean[others])
     assert not got[[3, 11]].isfinite().any()
     # A weight row that is not finite spoils its output column alone.
     w[7, 40] = float("nan")
-    got = kernels.mxfp4_linear(x[:2].cuda(), kernels.quantize_mxfp4(w.cuda()))
-    assert got[:, 7].isnan().all() and torch.equal(got[:, 8:], clean[:2, 8:])
+    got, clean = (kernels.mxfp4_linear(x[:2].cuda(), p) for p in (kernels.quantize_mxfp4(w.cuda()), q))
+    assert got[:, 7].isnan().all() and torch.equal(got[:, 8:], clean[:, 8:])
 
 
 def test_a_row_does_not_depend_on_its_neighbours() -> None:
@@ -292,12 +311,29 @@ def test_blocks_chained_by_the_residual_norm() -> None:
     assert float((out.float() - stepped.float()).norm() / stepped.float().norm()) <= 2.0**-7
 
 
-def test_graph_replay_and_two_streams() -> None:
+def test_the_c_entry_adds_into_the_residual() -> None:
+    from ce4b200 import _lib, kernels
+
+    g = torch.Generator().manual_seed(2)
+    q = kernels.quantize_mxfp4(_weight(300, 256, 6).cuda())
+    stream = torch.cuda.current_stream().cuda_stream
+    for rows in (5, 40):
+        x = torch.randn(rows, 256, generator=g).bfloat16().cuda()
+        residual = torch.randn(rows, 300, generator=g).bfloat16().cuda()
+        want = kernels.mxfp4_linear(x, q, residual=residual)
+        _lib.check(_lib.library().ce4b_mxfp4_linear(
+            x.data_ptr(), q.values.data_ptr(), q.scales.data_ptr(), residual.data_ptr(), residual.data_ptr(),
+            rows, 300, 256, stream))
+        assert torch.equal(residual, want)
+
+
+@pytest.mark.parametrize("rows", [9, 50])
+def test_graph_replay_and_two_streams(rows: int) -> None:
     from ce4b200 import kernels
 
     g = torch.Generator().manual_seed(13)
     q = kernels.quantize_mxfp4(_weight(384, 512, 3).cuda())
-    x = torch.randn(9, 512, generator=g).bfloat16().cuda()
+    x = torch.randn(rows, 512, generator=g).bfloat16().cuda()
     kernels.mxfp4_linear(x, q)
     torch.cuda.synchronize()
     graphs, outs = [], []
@@ -306,7 +342,7 @@ def test_graph_replay_and_two_streams() -> None:
         with torch.cuda.graph(graph):
             outs.append(kernels.mxfp4_linear(kernels.mxfp4_linear(x, q).repeat(1, 2)[:, :512].contiguous(), q))
         graphs.append(graph)
-    x.copy_(torch.randn(9, 512, generator=g).bfloat16())
+    x.copy_(torch.randn(rows, 512, generator=g).bfloat16())
     streams = [torch.cuda.Stream() for _ in range(2)]
     torch.cuda.synchronize()
     for _ in range(20):

@@ -32,7 +32,11 @@ def _formula(s: torch.Tensor, weight: torch.Tensor, eps: float = EPS) -> torch.T
 
 
 SIZES = [(1, 1), (1, 8), (1, 512), (3, 31), (2, 33), (5, 128), (7, 769), (64, 512), (130, 1000),
-         (9, 2048), (4, 4104), (3, 8192), (2, 8200), (2, 20000), (1, 65536), (1, 70001), (700, 128), (3000, 264)]
+         (9, 2048), (4, 4104), (3, 8192), (2, 8200), (2, 20000), (1, 65536), (1, 70001), (700, 128), (3000, 264),
+         # Rows enough for the blocks to take several in turn, at each of their widths.
+         (70000, 33), (30000, 100), (40001, 128), (14000, 250), (9601, 512), (9600, 509), (4000, 1000), (4000, 1001),
+         (2001, 2048), (2000, 2045), (1000, 4096), (1000, 4001), (500, 8192), (500, 8191), (300, 16384), (300, 16001),
+         (100, 32768), (100, 32001)]
 
 
 @pytest.mark.parametrize("rows,width", SIZES)
@@ -60,7 +64,8 @@ def test_without_a_residual_it_is_the_norm_of_x(rows: int, width: int) -> None:
 
 
 @pytest.mark.parametrize("rows,width", [(1, 128), (3, 512), (64, 512), (127, 384), (129, 2048), (256, 1024),
-                                        (2, 8192), (1, 16384), (300, 4224)])
+                                        (2, 8192), (1, 16384), (300, 4224), (9700, 512), (5000, 896), (1300, 2048),
+                                        (700, 4096), (330, 8192), (160, 16384), (90, 32768)])
 def test_mxfp8_output_equals_quantising_the_bf16_one(rows: int, width: int) -> None:
     from ce4b200 import kernels
     from oracle import mxfp8
