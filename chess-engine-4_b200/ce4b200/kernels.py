@@ -221,7 +221,7 @@ def add_rmsnorm_mxfp8(
     if width % MXFP8_TILE_SIZE:
         raise ValueError(f"x must have a multiple of {MXFP8_TILE_SIZE} columns")
     values = torch.empty_like(x, dtype=torch.float8_e4m3fn)
-    scales = torch.empty(-(-rows // 128), width // 128, 32, 16, dtype=torch.uint8, device=x.device)
+    scales = x.new_empty(-(-rows // 128), width // 128, 32, 16, dtype=torch.uint8)
     total = x if residual is None else torch.empty_like(x)
     _call(
         "ce4b_add_rmsnorm_mxfp8", x.get_device(), x.data_ptr(),
@@ -448,8 +448,8 @@ def quantize_mxfp4(weight: torch.Tensor) -> Mxfp4Tensor:
     rows, cols = weight.shape
     if cols % MXFP8_TILE_SIZE:
         raise ValueError(f"weight must have a multiple of {MXFP8_TILE_SIZE} columns")
-    values = torch.empty(rows, cols // 2, dtype=torch.uint8, device=weight.device)
-    scales = torch.empty(-(-rows // 128), cols // 128, 32, 16, dtype=torch.uint8, device=weight.device)
+    values = weight.new_empty(rows, cols // 2, dtype=torch.uint8)
+    scales = weight.new_empty(-(-rows // 128), cols // 128, 32, 16, dtype=torch.uint8)
     _call(
         "ce4b_quantize_mxfp4", weight.get_device(), weight.data_ptr(), values.data_ptr(),
         scales.data_ptr(), rows, cols,
@@ -462,7 +462,7 @@ def dequantize_mxfp4(weight: Mxfp4Tensor) -> torch.Tensor:
 
     rows, cols = _need_mxfp4("weight", weight)
     values = weight.values
-    out = torch.empty(rows, cols, dtype=torch.bfloat16, device=values.device)
+    out = values.new_empty(rows, cols, dtype=torch.bfloat16)
     _call(
         "ce4b_dequantize_mxfp4", values.get_device(), values.data_ptr(), weight.scales.data_ptr(),
         out.data_ptr(), rows, cols,
