@@ -111,16 +111,24 @@ __device__ __forceinline__ void store_chunk(bf16* p, const uint32_t (&v)[4], int
 // matrix: the row's first and last one hold elements of its neighbours, which are masked
 // after the load and left out of the store, and w is shifted to the row's offset.
 //
-// Bound by memory: 65536 x 1024 takes 83.5 us, 6.4 TB/s of the 6.56 a copy reaches. The MXFP8
-// form needs about 30 instructions an element and keeps the issue slots two thirds busy while
-// it streams: 16384 x 2048 takes 46.1 us (5.1 TB/s). Rows off 16 bytes pay their ends: 65536 x
-// 769 takes 91 us (4.4 TB/s). One row of 512 takes 1.6 us, a launch.
+// Blocks are as small as a row allows, so that their steps interleave: 256 threads for four rows
+// of 1021 x 769 took 4.4 us, 128 for one take 3.1; to MXFP8 65536 x 1024 took 83, takes 76.
+//
+// Bound by memory: 65536 x 1024 takes 84.9 us, 6.3 TB/s of the 6.56 a copy reaches, to MXFP8 76.8
+// (6.1 TB/s). Where the MXFP8 form's 28 instructions an element do not hide as well it stays
+// below: 16384 x 2048 takes 41.5 us (5.7 TB/s). Rows off 16 bytes pay their ends: 65536 x 769 takes
+// 88 us (4.6 TB/s). One row of 512 takes 1.5 us, a launch.
+template <int V, int TPR>
+constexpr int norm_threads() {
+  return TPR > (V >= 2 ? 32 : 64) ? TPR : (V >= 2 ? 32 : 64);
+}
+
 template <int V, int TPR, bool ALIGNED, bool MX>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
+__global__ void __launch_bounds__(norm_threads<V, TPR>())
     add_rmsnorm_kernel(const bf16* x, const bf16* residual, const bf16* __restrict__ w, bf16* sum,
                        bf16* out, uint8_t* codes, uint8_t* scales, int rows, int width,
                        double inv_width, float eps) {
-  constexpr int kThreads = TPR > 256 ? TPR : 256;
+  constexpr int kThreads = norm_threads<V, TPR>();
   constexpr int kRows = kThreads / TPR;  // rows of a block at a time
   constexpr int kWarps = TPR < 32 ? 1 : TPR / 32;  // warps of a row
   __shared__ double part[2][kThreads / 32];
@@ -128,7 +136,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
   grid_dependency_wait();
   grid_launch_dependents();
   // w is loaded ahead of the row's sum, or, where registers are short, at its use.
-  constexpr bool kKeepW = V <= 2 || (ALIGNED && V <= 4);
+  constexpr bool kKeepW = V <= 2;
   auto load_w = [&](int c, int shift) {  // columns c - shift .. + 7 of w
     if constexpr (ALIGNED) return *reinterpret_cast<const uint4*>(w + c);
     uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
@@ -343,7 +351,7 @@ struct NormArgs {
 
 template <int V, int TPR, bool ALIGNED, bool MX>
 void launch_norm(const NormArgs& a) {
-  constexpr int kThreads = TPR > 256 ? TPR : 256;
+  constexpr int kThreads = norm_threads<V, TPR>();
   constexpr int kRows = kThreads / TPR;
   const int64_t rows = MX ? (static_cast<int64_t>(a.rows) + 127) / 128 * 128 : a.rows;
   // Blocks that stay on the GPU (2048 threads an SM at most) and take rows in turn.
@@ -356,9 +364,10 @@ template <bool ALIGNED, bool MX>
 bool launch_rows(const NormArgs& a) {
   const int chunks = ALIGNED ? a.width / 8 : (a.width + 14) / 8;
   // Few rows: as many threads per row as it has chunks, for the shortest chain. Many rows: two
-  // chunks a thread (four where their ends cost), which keeps loads in flight and w in registers;
-  // us with 1 | 2 | 4 chunks: 16384 x 2048 54.2 | 43.3 | 50.4, 65536 x 1024 107 | 83.5 | 85.1,
-  // 10000 x 3001 - | 63.6 | 52.9. Rows wider than that are one block's with eight chunks a thread.
+  // chunks a thread, w beside them in registers; the MXFP8 form and rows off 16 bytes, which do
+  // more per row and thread, four, w read at its use. us with 1 | 2 | 4 chunks: 16384 x 2048 54.2 |
+  // 42.7 | 44.4, to MXFP8 60.8 | 45.8 | 41.5, 10000 x 3001 - | 63.6 | 50.0. Rows wider than 16384 are
+  // one block's with eight chunks a thread.
   const bool few = static_cast<int64_t>(a.rows) * chunks <= static_cast<int64_t>(sm_count()) * 2048;
   if (chunks <= 8) return launch_norm<1, 8, ALIGNED, MX>(a), true;
   if (chunks <= 16) return launch_norm<1, 16, ALIGNED, MX>(a), true;
@@ -372,10 +381,17 @@ bool launch_rows(const NormArgs& a) {
   }
   if (chunks <= 32) return launch_norm<1, 32, ALIGNED, MX>(a), true;
   if (chunks <= 64) return launch_norm<2, 32, ALIGNED, MX>(a), true;
-  if (chunks <= 128) return ALIGNED ? launch_norm<2, 64, ALIGNED, MX>(a) : launch_norm<4, 32, ALIGNED, MX>(a), true;
-  if (chunks <= 256) return ALIGNED ? launch_norm<2, 128, ALIGNED, MX>(a) : launch_norm<4, 64, ALIGNED, MX>(a), true;
-  if (chunks <= 512) return ALIGNED ? launch_norm<2, 256, ALIGNED, MX>(a) : launch_norm<4, 128, ALIGNED, MX>(a), true;
-  if (chunks <= 1024) return ALIGNED ? launch_norm<2, 512, ALIGNED, MX>(a) : launch_norm<4, 256, ALIGNED, MX>(a), true;
+  if constexpr (ALIGNED && !MX) {
+    if (chunks <= 128) return launch_norm<2, 64, ALIGNED, MX>(a), true;
+    if (chunks <= 256) return launch_norm<2, 128, ALIGNED, MX>(a), true;
+    if (chunks <= 512) return launch_norm<2, 256, ALIGNED, MX>(a), true;
+    if (chunks <= 1024) return launch_norm<2, 512, ALIGNED, MX>(a), true;
+  } else {
+    if (chunks <= 128) return launch_norm<4, 32, ALIGNED, MX>(a), true;
+    if (chunks <= 256) return launch_norm<4, 64, ALIGNED, MX>(a), true;
+    if (chunks <= 512) return launch_norm<4, 128, ALIGNED, MX>(a), true;
+    if (chunks <= 1024) return launch_norm<4, 256, ALIGNED, MX>(a), true;
+  }
   if (chunks <= 2048) return launch_norm<2, 1024, ALIGNED, MX>(a), true;
   if (chunks <= 4096) return launch_norm<8, 512, ALIGNED, MX>(a), true;
   return false;
