@@ -281,30 +281,31 @@ __global__ void __launch_bounds__(norm_threads<V, TPR>())
 
 // Any width, alignment and form, one block per row (rows in blockIdx.x): rows too wide for the
 // registers above, and matrices whose buffers start off 16 bytes. The row's sum is read again
-// (from the cache) for the second pass.
+// (from the cache) for the second pass. Columns are counted unsigned: the last one's successors
+// pass 2^31.
 __global__ void add_rmsnorm_any_kernel(const bf16* x, const bf16* residual, const bf16* w, bf16* sum,
                                        bf16* out, uint8_t* codes, uint8_t* scales, int rows,
-                                       int width, double inv_width, float eps) {
+                                       uint32_t width, double inv_width, float eps) {
   __shared__ double part[32];
   const int row = blockIdx.x;
   if (row >= rows) {  // padding rows of the last scale tile
-    for (int b = threadIdx.x; b < width / 32; b += blockDim.x) scales[mx_scale_offset(row, b, width / 128)] = 0;
+    for (uint32_t b = threadIdx.x; b < width / 32; b += blockDim.x) scales[mx_scale_offset(row, b, width / 128)] = 0;
     return;
   }
   const size_t at = static_cast<size_t>(row) * width;
   double ss = 0.0;
-  const int step = blockDim.x;
-  for (int c0 = threadIdx.x; c0 < width; c0 += 4 * step) {
+  const uint32_t step = blockDim.x;
+  for (uint32_t c0 = threadIdx.x; c0 < width; c0 += 4 * step) {
     float s[4], r[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int c = c0 + j * step;
+      const uint32_t c = c0 + j * step;
       s[j] = c < width ? __bfloat162float(x[at + c]) : 0.0f;
       r[j] = c < width && residual != nullptr ? __bfloat162float(residual[at + c]) : 0.0f;
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int c = c0 + j * step;
+      const uint32_t c = c0 + j * step;
       if (residual != nullptr && c < width) {
         s[j] = bf16_round(s[j] + r[j]);
         sum[at + c] = __float2bfloat16_rn(s[j]);
@@ -321,13 +322,13 @@ __global__ void add_rmsnorm_any_kernel(const bf16* x, const bf16* residual, cons
   const bf16* src = residual != nullptr ? sum : x;
   if (codes == nullptr) {
 #pragma unroll 4
-    for (int c = threadIdx.x; c < width; c += step) {
+    for (uint32_t c = threadIdx.x; c < width; c += step) {
       out[at + c] = __float2bfloat16_rn(
           scale_product(__bfloat162float(src[at + c]), __bfloat162float(w[c]), f));
     }
     return;
   }
-  for (int b = threadIdx.x; b < width / 32; b += blockDim.x) {
+  for (uint32_t b = threadIdx.x; b < width / 32; b += blockDim.x) {
     float v[32];
     for (int j = 0; j < 32; ++j) {
       v[j] = bf16_round(scale_product(__bfloat162float(src[at + b * 32 + j]), __bfloat162float(w[b * 32 + j]), f));

@@ -198,3 +198,30 @@ def test_mxfp8_blocks_of_a_ragged_batch(rows: int, d: int, h: int) -> None:
     assert q.values.shape == (rows, d)
     with pytest.raises(ValueError, match="padded"):
         kernels.mxfp8_gemm(kernels.Mxfp8Tensor(n.values[:1], n.scales[:0]), up)
+
+
+def test_a_row_of_the_largest_width() -> None:
+    """Column counters past 2^31 do not come back negative. The row repeats 2^16 values, so that
+    its statistics and its results are those of one period."""
+
+    from ce4b200 import kernels
+
+    width, period = 2**31 - 256, 2**16
+    whole = width // period * period
+    values, _, gains = _inputs(1, period, 11)
+
+    def repeated(v: torch.Tensor) -> torch.Tensor:
+        row = torch.empty(width, dtype=torch.bfloat16, device="cuda")
+        row[:whole].view(-1, period).copy_(v.view(1, -1).expand(whole // period, -1))
+        row[whole:] = v.flatten()[: width - whole]
+        return row
+
+    squares = values.double().square().flatten()
+    mean = (squares.sum() * (whole // period) + squares[: width - whole].sum()) / width
+    eps = float(torch.tensor(EPS, dtype=torch.float32))
+    expected = (values.double() / torch.sqrt(mean + eps) * gains.double()).float().bfloat16().flatten()
+    _, n = kernels.add_rmsnorm_forward(repeated(values)[None], None, repeated(gains))
+    n = n.flatten()
+    for start in range(0, whole, 2**28):
+        assert bool((n[start : min(start + 2**28, whole)].view(-1, period) == expected).all())
+    assert torch.equal(n[whole:], expected[: width - whole])
