@@ -582,6 +582,7 @@ int ce4b_mxfp8_gemm(const void* a_codes_dev, const void* a_scales_dev, const voi
   return guarded([&] {
     require(a_codes_dev && a_scales_dev && b_codes_dev && b_scales_dev && c_dev, "null pointer");
     require(m >= 1 && n >= 128 && k >= 128, "MXFP8 GEMM N and K must be at least 128");
+    require(m <= INT32_MAX - 127, "MXFP8 GEMM takes at most 2^31 - 128 rows");
     require(n % 128 == 0 && k % 128 == 0, "MXFP8 GEMM N and K must be multiples of 128");
     const CUtensorMap ta = make_tmap_u8(a_codes_dev, m, k, k, 128);
     const CUtensorMap tb = make_tmap_u8(b_codes_dev, n, k, k, 128);
@@ -594,6 +595,8 @@ int ce4b_mxfp8_gemm(const void* a_codes_dev, const void* a_scales_dev, const voi
 // ------------------------------------------------------------------ residual norm, MXFP4
 namespace {
 bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+// Kernels round extents up to whole tiles in 32 bits.
+constexpr int kMaxExtent = INT32_MAX - 255;
 }  // namespace
 
 int ce4b_add_rmsnorm(const void* x_dev, const void* residual_dev, const void* weight_dev,
@@ -602,6 +605,7 @@ int ce4b_add_rmsnorm(const void* x_dev, const void* residual_dev, const void* we
     require(x_dev && weight_dev && out_dev, "null pointer");
     require(residual_dev == nullptr || sum_dev != nullptr, "a residual needs an output for the sum");
     require(rows >= 1 && width >= 1, "extents must be positive");
+    require(rows <= kMaxExtent && width <= kMaxExtent, "extents are too large");
     add_rmsnorm_rows(static_cast<const bf16*>(x_dev), static_cast<const bf16*>(residual_dev),
                      static_cast<const bf16*>(weight_dev), static_cast<bf16*>(sum_dev),
                      static_cast<bf16*>(out_dev), nullptr, nullptr, rows, width, eps,
@@ -616,7 +620,7 @@ int ce4b_add_rmsnorm_mxfp8(const void* x_dev, const void* residual_dev, const vo
     require(x_dev && weight_dev && codes_dev && scales_dev, "null pointer");
     require(residual_dev == nullptr || sum_dev != nullptr, "a residual needs an output for the sum");
     require(rows >= 1 && width >= 1, "extents must be positive");
-    require(rows <= INT32_MAX - 127, "too many rows");
+    require(rows <= kMaxExtent && width <= kMaxExtent, "extents are too large");
     require(width % 128 == 0, "MXFP8 rows need a width that is a multiple of 128");
     require(aligned(codes_dev, 16), "MXFP8 codes must be 16-byte aligned");
     add_rmsnorm_rows(static_cast<const bf16*>(x_dev), static_cast<const bf16*>(residual_dev),
@@ -631,6 +635,7 @@ int ce4b_quantize_mxfp4(const void* x_dev, void* codes_dev, void* scales_dev, in
   return guarded([&] {
     require(x_dev && codes_dev && scales_dev, "null pointer");
     require(rows >= 1 && cols >= 1, "extents must be positive");
+    require(rows <= kMaxExtent && cols <= kMaxExtent, "extents are too large");
     require(cols % 128 == 0, "MXFP4 columns must be a multiple of 128");
     require(aligned(x_dev, 16) && aligned(codes_dev, 16) && aligned(scales_dev, 16),
             "MXFP4 buffers must be 16-byte aligned");
@@ -644,6 +649,7 @@ int ce4b_dequantize_mxfp4(const void* codes_dev, const void* scales_dev, void* o
   return guarded([&] {
     require(codes_dev && scales_dev && out_dev, "null pointer");
     require(rows >= 1 && cols >= 1, "extents must be positive");
+    require(rows <= kMaxExtent && cols <= kMaxExtent, "extents are too large");
     require(cols % 128 == 0, "MXFP4 columns must be a multiple of 128");
     require(aligned(codes_dev, 16) && aligned(scales_dev, 16) && aligned(out_dev, 16),
             "MXFP4 buffers must be 16-byte aligned");
@@ -658,6 +664,7 @@ int ce4b_mxfp4_linear(const void* x_dev, const void* codes_dev, const void* scal
   return guarded([&] {
     require(x_dev && codes_dev && scales_dev && out_dev, "null pointer");
     require(rows >= 1 && n >= 1 && k >= 1, "extents must be positive");
+    require(rows <= kMaxExtent && n <= kMaxExtent && k <= kMaxExtent, "extents are too large");
     require(k % 128 == 0, "MXFP4 columns must be a multiple of 128");
     require(aligned(x_dev, 16) && aligned(codes_dev, 16) && aligned(scales_dev, 16),
             "MXFP4 operands must be 16-byte aligned");
@@ -672,7 +679,8 @@ int ce4b_mxfp4_swiglu(const void* x_dev, const void* codes_dev, const void* scal
   return guarded([&] {
     require(x_dev && codes_dev && scales_dev && hidden_dev, "null pointer");
     require(rows >= 1 && hidden_dim >= 1 && k >= 1, "extents must be positive");
-    require(hidden_dim <= INT32_MAX / 2, "hidden_dim is too large");
+    require(rows <= kMaxExtent && k <= kMaxExtent, "extents are too large");
+    require(hidden_dim <= kMaxExtent / 2, "hidden_dim is too large");
     require(k % 128 == 0, "MXFP4 columns must be a multiple of 128");
     require(aligned(x_dev, 16) && aligned(codes_dev, 16) && aligned(scales_dev, 16),
             "MXFP4 operands must be 16-byte aligned");

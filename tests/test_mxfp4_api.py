@@ -145,3 +145,20 @@ def test_c_entries_check_on_the_host() -> None:
     refused(lib.ce4b_mxfp4_linear(p + 2, p, p, None, p, 1, 8, 128, None), "aligned")
     refused(lib.ce4b_mxfp4_swiglu(p, p + 4, p, p, 1, 8, 128, None), "aligned")
     refused(lib.ce4b_mxfp4_swiglu(p, p, p, p, 1, 2**30, 128, None), "too large")
+
+
+def test_c_entries_refuse_extents_that_would_wrap() -> None:
+    lib, bad, p, top = _lib.library(), _lib.CE4B_ERR_INVALID_ARGUMENT, 4096, 2**31 - 1
+
+    def refused(status: int) -> None:
+        assert status == bad and ("too large" in _lib.last_error() or "at most" in _lib.last_error())
+
+    refused(lib.ce4b_add_rmsnorm(p, None, p, None, p, 1, top, 1e-6, None))
+    refused(lib.ce4b_add_rmsnorm(p, None, p, None, p, top, 1, 1e-6, None))
+    refused(lib.ce4b_add_rmsnorm_mxfp8(p, None, p, None, p, p, top, 128, 1e-6, None))
+    refused(lib.ce4b_quantize_mxfp4(p, p, p, top, 128, None))
+    refused(lib.ce4b_dequantize_mxfp4(p, p, p, top, 128, None))
+    refused(lib.ce4b_mxfp4_linear(p, p, p, None, p, 1, top, 128, None))
+    refused(lib.ce4b_mxfp4_linear(p, p, p, None, p, top, 8, 128, None))
+    refused(lib.ce4b_mxfp4_swiglu(p, p, p, p, 1, top // 2, 128, None))
+    refused(lib.ce4b_mxfp8_gemm(p, p, p, p, p, top, 128, 128, None))
