@@ -37,12 +37,13 @@ __device__ __forceinline__ uint32_t max_abs_bf16x2(uint32_t a, uint32_t b) {
 // bytes of BF16, 4 bytes of codes), and kTiles column tiles at once for loads in flight. Sixteen
 // threads hold the four scale bytes of a row in a tile, one 32-bit word. Bound by memory: 8192 x
 // 8192 there and back takes 61.5 us, 5.5 TB/s of the bytes in and out and of the 4-bit form
-// between them (which the L2 cache mostly holds).
+// between them (which the L2 cache mostly holds). No pointer is declared unaliased: the loads would
+// become read-only ones, which a kernel may not use for what its predecessor still writes when
+// it starts.
 constexpr int kTiles = 4;
 
 __global__ void __launch_bounds__(256)
-    mx4_quantize_kernel(const bf16* __restrict__ x, uint8_t* __restrict__ codes,
-                        uint8_t* __restrict__ scales, int rows, int cols) {
+    mx4_quantize_kernel(const bf16* x, uint8_t* codes, uint8_t* scales, int rows, int cols) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16;
   const int lane = threadIdx.x % 16;
   const int col_tiles = cols / 128;
@@ -90,8 +91,8 @@ __global__ void __launch_bounds__(256)
 }
 
 __global__ void __launch_bounds__(256)
-    mx4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                          bf16* __restrict__ out, int rows, int cols) {
+    mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, bf16* out, int rows,
+                          int cols) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16;
   const int lane = threadIdx.x % 16;
   const int col_tiles = cols / 128;

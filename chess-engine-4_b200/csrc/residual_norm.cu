@@ -118,6 +118,7 @@ __device__ __forceinline__ void store_chunk(bf16* p, const uint32_t (&v)[4], int
 // (6.1 TB/s). Where the MXFP8 form's 28 instructions an element do not hide as well it stays
 // below: 16384 x 2048 takes 41.5 us (5.7 TB/s). Rows off 16 bytes pay their ends: 65536 x 769 takes
 // 88 us (4.6 TB/s). One row of 512 takes 1.5 us, a launch.
+// w too may be what the predecessor writes while this kernel starts, so it takes ordinary loads.
 template <int V, int TPR>
 constexpr int norm_threads() {
   return TPR > (V >= 2 ? 32 : 64) ? TPR : (V >= 2 ? 32 : 64);
@@ -125,7 +126,7 @@ constexpr int norm_threads() {
 
 template <int V, int TPR, bool ALIGNED, bool MX>
 __global__ void __launch_bounds__(norm_threads<V, TPR>())
-    add_rmsnorm_kernel(const bf16* x, const bf16* residual, const bf16* __restrict__ w, bf16* sum,
+    add_rmsnorm_kernel(const bf16* x, const bf16* residual, const bf16* w, bf16* sum,
                        bf16* out, uint8_t* codes, uint8_t* scales, int rows, int width,
                        double inv_width, float eps) {
   constexpr int kThreads = norm_threads<V, TPR>();

@@ -352,3 +352,34 @@ def test_graph_replay_and_two_streams(rows: int) -> None:
     torch.cuda.synchronize()
     want = kernels.mxfp4_linear(kernels.mxfp4_linear(x, q).repeat(1, 2)[:, :512].contiguous(), q)
     assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+def test_every_operand_may_come_from_the_kernel_before() -> None:
+    """Kernels start under their predecessor's tail; what it writes last, a norm weight or a
+    quantised matrix included, is read after it."""
+
+    from ce4b200 import kernels
+
+    g = torch.Generator().manual_seed(5)
+    base = torch.randn(2048, 1024, generator=g).bfloat16().cuda()
+
+    def chain(x: torch.Tensor, wait: bool) -> list[torch.Tensor]:
+        pause = torch.cuda.synchronize if wait else lambda: None
+        _, n = kernels.add_rmsnorm_forward(x, None, x[0])
+        pause()
+        _, n2 = kernels.add_rmsnorm_forward(n, x, n[-1])  # the weight: the rows written last
+        pause()
+        packed = kernels.quantize_mxfp4(n2)
+        pause()
+        back = kernels.dequantize_mxfp4(packed)
+        pause()
+        total, _ = kernels.add_rmsnorm_mxfp8(back, n2, back[-1])
+        pause()
+        y = kernels.mxfp4_linear(total[-3:].contiguous(), packed)
+        pause()
+        return [n, n2, packed.values, packed.scales, back, total, y]
+
+    for i in range(8):
+        x = base.roll(i, 0) * (i + 1)
+        for a, b in zip(chain(x, False), chain(x, True), strict=True):
+            assert torch.equal(a, b)
