@@ -160,17 +160,21 @@ def _call(name: str, index: int, *args: object) -> None:
 
 def _need_norm_operands(
     x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor
-) -> None:
-    if _is_bf16_matrix(x) and weight.is_cuda and weight.dtype is torch.bfloat16:
-        shape, index = x.shape, x.get_device()
+) -> torch.Size:
+    shape, bf16 = x.shape, torch.bfloat16
+    if x.is_cuda and x.dtype is bf16 and len(shape) == 2 and x.is_contiguous():
+        rows, width = shape
+        index = x.get_device()
         if (
-            weight.shape == shape[1:] and weight.is_contiguous() and weight.get_device() == index
+            1 <= rows <= _MAX_EXTENT and 1 <= width <= _MAX_EXTENT
+            and weight.get_device() == index and weight.dtype is bf16 and weight.shape == (width,)
+            and weight.is_contiguous()
             and (residual is None or (
-                residual.is_cuda and residual.dtype is torch.bfloat16 and residual.is_contiguous()
-                and residual.shape == shape and residual.get_device() == index
+                residual.get_device() == index and residual.dtype is bf16
+                and residual.shape == shape and residual.is_contiguous()
             ))
         ):
-            return
+            return shape
     _need_bf16_matrix("x", x)
     if residual is not None:
         _need_bf16_matrix("residual", residual)
@@ -181,6 +185,7 @@ def _need_norm_operands(
     _check_bf16_vector("weight", weight, x.shape[1])
     if not _same_device(weight, x):
         raise ValueError("weight must be on x's device")
+    return shape
 
 
 def add_rmsnorm_forward(
@@ -195,13 +200,13 @@ def add_rmsnorm_forward(
     returned as the sum. BF16 rows of any width.
     """
 
-    _need_norm_operands(x, residual, weight)
+    rows, width = _need_norm_operands(x, residual, weight)
     out = torch.empty_like(x)
     total = x if residual is None else torch.empty_like(x)
     _call(
         "ce4b_add_rmsnorm", x.get_device(), x.data_ptr(),
         None if residual is None else residual.data_ptr(), weight.data_ptr(), total.data_ptr(),
-        out.data_ptr(), x.shape[0], x.shape[1], eps,
+        out.data_ptr(), rows, width, eps,
     )
     return total, out
 
@@ -216,8 +221,7 @@ def add_rmsnorm_mxfp8(
     rows with zero bytes, and :func:`mxfp8_gemm` takes such a left operand).
     """
 
-    _need_norm_operands(x, residual, weight)
-    rows, width = x.shape
+    rows, width = _need_norm_operands(x, residual, weight)
     if width % MXFP8_TILE_SIZE:
         raise ValueError(f"x must have a multiple of {MXFP8_TILE_SIZE} columns")
     values = torch.empty_like(x, dtype=torch.float8_e4m3fn)
@@ -416,11 +420,21 @@ def _need_mxfp4(name: str, weight: Mxfp4Tensor, x: torch.Tensor | None = None) -
     if not isinstance(weight, Mxfp4Tensor):
         raise ValueError(f"{name} must be an Mxfp4Tensor")
     values, scales = weight.values, weight.scales
-    if not (values.is_cuda and values.dtype is torch.uint8 and values.dim() == 2 and values.is_contiguous()):
-        if values.device.type != "cuda" or values.dtype != torch.uint8:
-            raise ValueError(f"{name} values must be a uint8 CUDA tensor")
-        if values.ndim != 2 or not values.is_contiguous():
-            raise ValueError(f"{name} values must be a contiguous matrix")
+    shape, u8 = values.shape, torch.uint8
+    if values.is_cuda and values.dtype is u8 and len(shape) == 2 and values.is_contiguous():
+        rows, half = shape
+        index = values.get_device()
+        if (
+            1 <= rows <= _MAX_EXTENT and 64 <= half <= _MAX_EXTENT // 2 and half % 64 == 0
+            and scales.get_device() == index and scales.dtype is u8
+            and scales.shape == (-(-rows // 128), half // 64, 32, 16) and scales.is_contiguous()
+            and (x is None or x.get_device() == index)
+        ):
+            return rows, 2 * half
+    if values.device.type != "cuda" or values.dtype != torch.uint8:
+        raise ValueError(f"{name} values must be a uint8 CUDA tensor")
+    if values.ndim != 2 or not values.is_contiguous():
+        raise ValueError(f"{name} values must be a contiguous matrix")
     rows, half = values.shape
     cols = 2 * half
     if not (1 <= rows <= _MAX_EXTENT and 1 <= cols <= _MAX_EXTENT):
@@ -480,8 +494,8 @@ def mxfp4_linear(
 
     _need_bf16_matrix("x", x)
     n, k = _need_mxfp4("weight", weight, x)
-    rows = x.shape[0]
-    if x.shape[1] != k:
+    rows, columns = x.shape
+    if columns != k:
         raise ValueError("MXFP4 product reduction dimensions do not match")
     if residual is not None:
         _need_bf16_matrix("residual", residual)
@@ -503,8 +517,8 @@ def mxfp4_swiglu(x: torch.Tensor, gate_up_weight: Mxfp4Tensor) -> torch.Tensor:
 
     _need_bf16_matrix("x", x)
     wide, k = _need_mxfp4("gate_up_weight", gate_up_weight, x)
-    rows = x.shape[0]
-    if x.shape[1] != k:
+    rows, columns = x.shape
+    if columns != k:
         raise ValueError("MXFP4 product reduction dimensions do not match")
     if wide % 2:
         raise ValueError("gate_up_weight must have an even number of rows")
