@@ -112,11 +112,11 @@ __device__ __forceinline__ void store_chunk(bf16* p, const uint32_t (&v)[4], int
 // after the load and left out of the store, and w is shifted to the row's offset.
 //
 // Blocks are as small as a row allows, so that their steps interleave: 256 threads for four rows
-// of 1021 x 769 took 4.4 us, 128 for one take 3.1; to MXFP8 65536 x 1024 took 83, takes 76.
+// of 1021 x 769 took 4.4 us, 128 for one take 3.1; to MXFP8 65536 x 1024 took 83, takes 77.
 //
-// Bound by memory: 65536 x 1024 takes 84.9 us, 6.3 TB/s of the 6.56 a copy reaches, to MXFP8 76.8
+// Bound by memory: 65536 x 1024 takes 85.2 us, 6.3 TB/s of the 6.56 a copy reaches, to MXFP8 77.1
 // (6.1 TB/s). Where the MXFP8 form's 28 instructions an element do not hide as well it stays
-// below: 16384 x 2048 takes 41.5 us (5.7 TB/s). Rows off 16 bytes pay their ends: 65536 x 769 takes
+// below: 16384 x 2048 takes 42.0 us (5.6 TB/s). Rows off 16 bytes pay their ends: 65536 x 769 takes
 // 88 us (4.6 TB/s). One row of 512 takes 1.5 us, a launch.
 // w too may be what the predecessor writes while this kernel starts, so it takes ordinary loads.
 template <int V, int TPR>
