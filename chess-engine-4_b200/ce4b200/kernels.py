@@ -374,6 +374,18 @@ def quantize_mxfp8_transpose(tensor: torch.Tensor) -> Mxfp8Tensor:
     return Mxfp8Tensor(values=values, scales=scales)
 
 
+def _check_mx_scales(tensor: Mxfp8Tensor) -> None:
+    # The GEMM copies 512 bytes per scale tile from this tensor, whatever it holds.
+    rows, cols = tensor.values.shape
+    scales, shape = tensor.scales, (-(-rows // 128), cols // 128, 32, 16)
+    if scales.dtype not in (torch.uint8, torch.float8_e8m0fnu):
+        raise ValueError("MXFP8 scales must have dtype torch.uint8")
+    if scales.shape != shape:
+        raise ValueError(f"MXFP8 scale tiles must be padded to 128 rows: {list(shape)}")
+    if not scales.is_contiguous() or not _same_device(scales, tensor.values):
+        raise ValueError("MXFP8 scales must be contiguous and on the values' device")
+
+
 def mxfp8_gemm(left: Mxfp8Tensor, right: Mxfp8Tensor) -> torch.Tensor:
     """``dequant(left) @ dequant(right).T`` in BF16 on block-scaled tcgen05 MMAs
     (replaces kernels/dense.py:87-113; any output width divisible by 128, and any number of
@@ -387,10 +399,12 @@ def mxfp8_gemm(left: Mxfp8Tensor, right: Mxfp8Tensor) -> torch.Tensor:
     for t in (left.values, right.values):
         if t.device.type != "cuda" or t.dtype != torch.float8_e4m3fn or not t.is_contiguous():
             raise ValueError("MXFP8 values must be contiguous float8_e4m3fn CUDA tensors")
+    if not _same_device(left.values, right.values):
+        raise ValueError("MXFP8 GEMM operands must be on one device")
     if rows < 1 or out_cols % 128 or reduction % 128:
         raise ValueError("MXFP8 GEMM columns and reduction must be multiples of 128")
-    if rows % 128 and left.scales.shape != (-(-rows // 128), reduction // 128, 32, 16):
-        raise ValueError("MXFP8 scale tiles of a ragged operand must be padded to 128 rows")
+    for t in (left, right):
+        _check_mx_scales(t)
     out = torch.empty(rows, out_cols, dtype=torch.bfloat16, device=left.values.device)
     with torch.cuda.device(out.device):
         _lib.check(
