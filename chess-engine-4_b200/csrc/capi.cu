@@ -557,6 +557,10 @@ int ce4b_moe_forward(const void* x_dev, const void* gate_up_weight_dev,
 }
 
 // ------------------------------------------------------------------ MXFP8 kernel ops
+namespace {
+bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+}  // namespace
+
 int ce4b_quantize_mxfp8(const void* x_dev, void* codes_dev, void* scales_dev, int rows, int cols,
                         void* stream) {
   return guarded([&] {
@@ -584,6 +588,10 @@ int ce4b_mxfp8_gemm(const void* a_codes_dev, const void* a_scales_dev, const voi
     require(m >= 1 && n >= 128 && k >= 128, "MXFP8 GEMM N and K must be at least 128");
     require(m <= INT32_MAX - 127, "MXFP8 GEMM takes at most 2^31 - 128 rows");
     require(n % 128 == 0 && k % 128 == 0, "MXFP8 GEMM N and K must be multiples of 128");
+    // Codes and C go through tensor maps, scale tiles through bulk copies.
+    require(aligned(a_codes_dev, 16) && aligned(a_scales_dev, 16) && aligned(b_codes_dev, 16) &&
+                aligned(b_scales_dev, 16) && aligned(c_dev, 16),
+            "MXFP8 GEMM operands must be 16-byte aligned");
     const CUtensorMap ta = make_tmap_u8(a_codes_dev, m, k, k, 128);
     const CUtensorMap tb = make_tmap_u8(b_codes_dev, n, k, k, 128);
     const CUtensorMap tc = make_tmap_bf16(c_dev, m, n, n, 128);
@@ -594,7 +602,6 @@ int ce4b_mxfp8_gemm(const void* a_codes_dev, const void* a_scales_dev, const voi
 
 // ------------------------------------------------------------------ residual norm, MXFP4
 namespace {
-bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 // Kernels round extents up to whole tiles in 32 bits.
 constexpr int kMaxExtent = INT32_MAX - 255;
 }  // namespace

@@ -408,8 +408,9 @@ int ce4b_quantize_mxfp8_transpose(const void* x_dev, void* codes_dev, void* scal
 /* C[M,N] BF16 = sum over 32-element K blocks of (A codes * 2^(sa-127)) (B codes *
  * 2^(sb-127)), FP32 accumulate: A, B E4M3 codes [M,K], [N,K] with scales in the
  * ce4b_quantize_mxfp8 layout; N and K multiples of 128, any M >= 1 (A's scale tiles cover
- * ceil(M/128)*128 rows, as ce4b_add_rmsnorm_mxfp8 writes them). Block-scaled tcgen05 MMA
- * (kind::mxf8f6f4). Replaces mxfp8_gemm (src/chess_engine_4/kernels/dense.py:87-113). */
+ * ceil(M/128)*128 rows, as ce4b_add_rmsnorm_mxfp8 writes them); every buffer 16-byte
+ * aligned. Block-scaled tcgen05 MMA (kind::mxf8f6f4). Replaces mxfp8_gemm
+ * (src/chess_engine_4/kernels/dense.py:87-113). */
 int ce4b_mxfp8_gemm(const void* a_codes_dev, const void* a_scales_dev, const void* b_codes_dev,
                     const void* b_scales_dev, void* c_dev, int m, int n, int k, void* stream);
 

@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from ce4b200 import kernels
+from ce4b200 import _lib, kernels
 
 
 class _Fake(torch.Tensor):
@@ -60,3 +60,14 @@ def test_scales_that_do_not_belong_to_the_right_values(scales, match: str) -> No
 def test_operands_on_two_devices() -> None:
     with pytest.raises(ValueError, match="one device"):
         kernels.mxfp8_gemm(_operand(128, 256), _operand(128, 256, where=("cuda", 1)))
+
+
+def test_the_c_entry_refuses_addresses_that_its_copies_cannot_take() -> None:
+    """Scale tiles travel in bulk copies, which fault off 16 bytes."""
+
+    lib, p = _lib.library(), 4096
+    for i in range(5):
+        for off in (1, 2, 4, 8):
+            args = [p + off * (j == i) for j in range(5)]
+            assert lib.ce4b_mxfp8_gemm(*args, 128, 128, 128, None) == _lib.CE4B_ERR_INVALID_ARGUMENT
+            assert "aligned" in _lib.last_error()
