@@ -604,6 +604,13 @@ int ce4b_mxfp8_gemm(const void* a_codes_dev, const void* a_scales_dev, const voi
 namespace {
 // Kernels round extents up to whole tiles in 32 bits.
 constexpr int kMaxExtent = INT32_MAX - 255;
+
+// Buffers of single BF16 elements (null is aligned).
+void require_elements(const void* a, const void* b = nullptr, const void* c = nullptr,
+                      const void* d = nullptr, const void* e = nullptr) {
+  require(aligned(a, 2) && aligned(b, 2) && aligned(c, 2) && aligned(d, 2) && aligned(e, 2),
+          "BF16 buffers must be 2-byte aligned");
+}
 }  // namespace
 
 int ce4b_add_rmsnorm(const void* x_dev, const void* residual_dev, const void* weight_dev,
@@ -613,6 +620,7 @@ int ce4b_add_rmsnorm(const void* x_dev, const void* residual_dev, const void* we
     require(residual_dev == nullptr || sum_dev != nullptr, "a residual needs an output for the sum");
     require(rows >= 1 && width >= 1, "extents must be positive");
     require(rows <= kMaxExtent && width <= kMaxExtent, "extents are too large");
+    require_elements(x_dev, residual_dev, weight_dev, sum_dev, out_dev);
     add_rmsnorm_rows(static_cast<const bf16*>(x_dev), static_cast<const bf16*>(residual_dev),
                      static_cast<const bf16*>(weight_dev), static_cast<bf16*>(sum_dev),
                      static_cast<bf16*>(out_dev), nullptr, nullptr, rows, width, eps,
@@ -630,6 +638,7 @@ int ce4b_add_rmsnorm_mxfp8(const void* x_dev, const void* residual_dev, const vo
     require(rows <= kMaxExtent && width <= kMaxExtent, "extents are too large");
     require(width % 128 == 0, "MXFP8 rows need a width that is a multiple of 128");
     require(aligned(codes_dev, 16), "MXFP8 codes must be 16-byte aligned");
+    require_elements(x_dev, residual_dev, weight_dev, sum_dev);
     add_rmsnorm_rows(static_cast<const bf16*>(x_dev), static_cast<const bf16*>(residual_dev),
                      static_cast<const bf16*>(weight_dev), static_cast<bf16*>(sum_dev), nullptr,
                      static_cast<uint8_t*>(codes_dev), static_cast<uint8_t*>(scales_dev), rows,
@@ -675,6 +684,7 @@ int ce4b_mxfp4_linear(const void* x_dev, const void* codes_dev, const void* scal
     require(k % 128 == 0, "MXFP4 columns must be a multiple of 128");
     require(aligned(x_dev, 16) && aligned(codes_dev, 16) && aligned(scales_dev, 16),
             "MXFP4 operands must be 16-byte aligned");
+    require_elements(residual_dev, out_dev);
     mx4_product(static_cast<const bf16*>(x_dev), static_cast<const uint8_t*>(codes_dev),
                 static_cast<const uint8_t*>(scales_dev), static_cast<const bf16*>(residual_dev),
                 static_cast<bf16*>(out_dev), rows, n, k, false, as_stream(stream));
@@ -691,6 +701,7 @@ int ce4b_mxfp4_swiglu(const void* x_dev, const void* codes_dev, const void* scal
     require(k % 128 == 0, "MXFP4 columns must be a multiple of 128");
     require(aligned(x_dev, 16) && aligned(codes_dev, 16) && aligned(scales_dev, 16),
             "MXFP4 operands must be 16-byte aligned");
+    require_elements(hidden_dev);
     mx4_product(static_cast<const bf16*>(x_dev), static_cast<const uint8_t*>(codes_dev),
                 static_cast<const uint8_t*>(scales_dev), nullptr, static_cast<bf16*>(hidden_dev),
                 rows, hidden_dim, k, true, as_stream(stream));

@@ -162,3 +162,21 @@ def test_c_entries_refuse_extents_that_would_wrap() -> None:
     refused(lib.ce4b_mxfp4_linear(p, p, p, None, p, top, 8, 128, None))
     refused(lib.ce4b_mxfp4_swiglu(p, p, p, p, 1, top // 2, 128, None))
     refused(lib.ce4b_mxfp8_gemm(p, p, p, p, p, top, 128, 128, None))
+
+
+def test_c_entries_refuse_addresses_between_elements() -> None:
+    """Any alignment of the elements: an address off two bytes holds no BF16 element."""
+
+    lib, bad, p = _lib.library(), _lib.CE4B_ERR_INVALID_ARGUMENT, 4096
+
+    def refused(status: int) -> None:
+        assert status == bad and "2-byte aligned" in _lib.last_error()
+
+    for i in range(5):
+        x, residual, w, total, out = (p + (j == i) for j in range(5))
+        refused(lib.ce4b_add_rmsnorm(x, residual, w, total, out, 1, 8, 1e-6, None))
+        if i < 4:
+            refused(lib.ce4b_add_rmsnorm_mxfp8(x, residual, w, total, p, p, 1, 128, 1e-6, None))
+    refused(lib.ce4b_mxfp4_linear(p, p, p, p + 1, p, 1, 8, 128, None))
+    refused(lib.ce4b_mxfp4_linear(p, p, p, None, p + 1, 1, 8, 128, None))
+    refused(lib.ce4b_mxfp4_swiglu(p, p, p, p + 1, 1, 8, 128, None))
