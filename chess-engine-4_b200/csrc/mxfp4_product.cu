@@ -14,9 +14,12 @@
 // the K blocks of one row tile, so that weights of few rows still occupy the GPU; their FP32
 // partial sums are added through distributed shared memory in rank order (deterministic).
 //
-// Bound: 64 rows, n = 28672, k = 8192 takes 61 us (125 MB of weight, 2.1 TB/s, 0.49 PFLOP/s): a K
-// block costs an SM 0.3 us of expansion, MMA and hand-over, where its bytes take 0.2. Small
-// weights pay the chain through one CTA, about 6 us (64 rows, n = 1024, k = 4096: 8.1 us).
+// Bound, at 64 rows: a launch whose CTAs have four K blocks each takes 6.6 us (n = 1024, k = 512),
+// 9.7 with two CTAs on every SM (n = 37888, k = 512); every further K block of an SM 0.43 us of
+// expansion, MMA and hand-over, where its bytes take 0.2 (n = 37888, k = 8192: 60.9 us). n = 28672,
+// k = 8192 takes 61 us too (125 MB of weight, 2.1 TB/s, 0.49 PFLOP/s), because its 224 row tiles
+// fill 76 SMs with two CTAs and leave one to each of the other 72. n = 1024, k = 4096, split over
+// clusters of eight, takes 8.1 us.
 #include <algorithm>
 
 #include "internal.h"
@@ -312,9 +315,11 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 // CTAs per row tile: as many as fit on the GPU at once (two an SM), with at least four K blocks
-// each. A CTA costs about 6 us beside its blocks (tensor memory, first bytes, join), 0.3 to 0.4
-// us each, so that a second wave never pays: 33 rows, n = 8192 (SwiGLU), k = 2048 takes 13.9 us
-// unsplit, 12.9 at 2 and 19.4 at 3, the first split of more CTAs than fit.
+// each. A launch costs about 5 us beside its blocks (tensor memory, first bytes, join), 0.43 us
+// each, so that a second wave never pays: 33 rows, n = 8192 (SwiGLU), k = 2048 takes 13.9 us
+// unsplit, 12.9 at 2 and 19.4 at 3, the first split of more CTAs than fit. A whole number of CTAs
+// a tile leaves SMs with one CTA beside others with two: with 149 to 295 tiles, unsplit, the time
+// is that of 296.
 int choose_split(int64_t tiles, int kblocks) {
   const int fit = static_cast<int>(2 * sm_count() / tiles);
   return std::max(1, std::min({kMaxSplit, fit, kblocks / 4}));

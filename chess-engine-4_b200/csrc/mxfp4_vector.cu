@@ -13,10 +13,12 @@
 // (deterministic).
 //
 // 1 row, n = 512, k = 1536: 2.2 us, of which the launch is 1.5. 7 rows, n = 28672, k = 8192:
-// 39.7 us (125 MB of weight, 3.2 TB/s), bound by the instructions of the expansion and by x's
-// 64-byte pieces in the load pipeline. (x resident in shared memory with one CTA of 16 warps per
-// SM and codes by asynchronous copies: 44 us; the tensor core's own E2M1 operand, which needs x
-// in 8-bit terms made by a second kernel: 50 us.)
+// 39.8 us (125 MB of weight, 3.2 TB/s), twice its bytes' time with no unit full: the load pipeline,
+// busy 73 %, also takes x's 64-byte pieces, a scale byte for each 16 bytes of codes and the spills
+// of the form used there (eight rows, two tiles a warp), which is held to 64 registers for four
+// CTAs an SM and spills 72 bytes a thread; one tile's codes are in flight per warp. (x resident in
+// shared memory with one CTA of 16 warps per SM and codes by asynchronous copies: 44 us; the
+// tensor core's own E2M1 operand, which needs x in 8-bit terms made by a second kernel: 50 us.)
 #include <algorithm>
 
 #include "internal.h"
@@ -195,9 +197,14 @@ void choose_tiles(const bf16* x, const uint8_t* codes, const uint8_t* scales, co
 }
 
 // Up to 16 rows this form is the faster one at every size. With 17 to 32 rows the MMAs and x's
-// fragments weigh more than the codes, and the tcgen05 form wins once its fixed 5 us are
-// spread over enough codes: 32 rows, codes in millions, this form | tcgen05 (us): 0.8 4.5 | 5.1,
-// 1.6 3.4 | 4.7, 4.2 8.5 | 6.6, 16.8 10.4 | 9.6, 235 100 | 63.
+// fragments weigh more than the codes, and the tcgen05 form wins once its fixed 6 us are
+// spread over enough codes. us, this form | tcgen05, n x k:
+//            512 x 1536  1024 x 2048  2048 x 2048  1024 x 4096  4096 x 4096  28672 x 8192
+//   17 rows  3.5 | 6.3   4.2 | 6.2    4.5 | 6.2    6.5 | 6.4    9.1 | 9.1    92 | 53
+//   24 rows  3.8 | 6.5   4.7 | 6.2    4.8 | 6.3    6.8 | 6.5    9.6 | 9.2    92 | 53
+//   32 rows  4.3 | 6.6   5.2 | 6.6    5.4 | 6.6    8.0 | 6.6    10.4 | 9.5   101 | 53
+// The limit is 2^21 codes. Between 2 and 4 million the better form also depends on k (eight warps
+// share k here), which the rule leaves out.
 template <bool SWIGLU>
 void product(const bf16* x, const uint8_t* codes, const uint8_t* scales, const bf16* residual,
              bf16* out, int rows, int n, int k, cudaStream_t s) {

@@ -13,10 +13,11 @@ namespace ce4b {
 namespace {
 
 // n is the BF16 rounding of the formula's FP32 value: the squares (exact in 64 bits) are summed
-// in 64 bits and the factor (mean + eps)^(-1/2) is kept as an FP32 pair hi + lo, so that a row's
-// result does not depend on the order of its sum, on the launch shape or on the row's
-// neighbours. Every form of the operator gives the same n, and the MXFP8 form quantises
-// exactly that value.
+// in 64 bits and the factor (mean + eps)^(-1/2) is kept as an FP32 pair hi + lo. A row's result
+// then depends neither on its neighbours nor on the order of its sum, which goes with the launch
+// shape, unless the formula's value lies within about 2^-40 (relative) of a border between two
+// BF16 values: a 64-bit sum of squares over more than 53 binades rounds too. The MXFP8 form
+// quantises the BF16 n.
 struct RowScale {
   float power;   // 2^e, about the factor's size
   float hi, lo;  // factor / 2^e = hi + lo, lo >= 0
@@ -42,7 +43,9 @@ __device__ __forceinline__ RowScale row_scale(double sum, double inv_width, floa
 
 // s * factor * w rounded to FP32 once. s * 2^e is exact and of the size of s * factor, so its
 // product with w (eight bits each: exact) overflows only where the result does; the last FMA
-// rounds the exact p * hi plus p * lo.
+// rounds the exact p * hi plus p * lo. Values under FP32's normal numbers, 2^-126, are the
+// exception: s * 2^e and p are multiples of 2^-149 there, so that an s over 2^142 below its row's
+// size loses bits and one over 2^150 below counts as 0, however large w is, as in any FP32 form.
 __device__ __forceinline__ float scale_product(float s, float w, const RowScale& f) {
   const float p = s * f.power * w;
   return fmaf(p, f.hi, p * f.lo);
@@ -356,7 +359,9 @@ void launch_norm(const NormArgs& a) {
   constexpr int kThreads = norm_threads<V, TPR>();
   constexpr int kRows = kThreads / TPR;
   const int64_t rows = MX ? (static_cast<int64_t>(a.rows) + 127) / 128 * 128 : a.rows;
-  // Blocks that stay on the GPU (2048 threads an SM at most) and take rows in turn.
+  // Blocks that take rows in turn, 2048 threads an SM. The forms for many rows use 54 to 64
+  // registers a thread, so that about half of these blocks are on the GPU at once and the others
+  // follow as they leave; a block for every row was slower.
   const int64_t grid = std::min<int64_t>((rows + kRows - 1) / kRows, static_cast<int64_t>(sm_count()) * (2048 / kThreads));
   launch(add_rmsnorm_kernel<V, TPR, ALIGNED, MX>, dim3(static_cast<unsigned>(grid)), kThreads, 0, 0, a.s,
          a.x, a.residual, a.w, a.sum, a.out, a.codes, a.scales, a.rows, a.width, 1.0 / a.width, a.eps);

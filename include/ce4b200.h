@@ -434,8 +434,10 @@ int ce4b_dense_block_forward_static(const void* x_dev, const void* norm_weight_d
 /* The residual addition and the RMSNorm after it, one pass: sum = bf16(x + residual) and
  * out = bf16(sum * (mean(sum^2) + eps)^(-1/2) * w) per row of [rows, width]. The squares are
  * summed in 64 bits and out is rounded from the formula's FP32 value, so a row's result
- * depends on neither the launch nor its neighbours. residual_dev may be NULL: the norm of x, and sum_dev is not
- * written (and may be NULL). sum_dev may be x_dev or residual_dev itself, the buffers
+ * depends on neither the launch nor its neighbours, but for values within about 2^-40
+ * (relative) of a border between two BF16 values. A sum element over 2^142 below its row's
+ * size loses bits (sum * factor leaves FP32's normal numbers). residual_dev may be NULL: the norm of x, and sum_dev is
+ * not written (and may be NULL). sum_dev may be x_dev or residual_dev itself, the buffers
  * overlap in no other way. Any alignment of the elements; rows, width >= 1. A NaN or an
  * infinity in a row makes that row's out NaN (0 where the row's other values are finite beside
  * an infinity). No counterpart in the reference, which adds and normalises in two launches
@@ -471,13 +473,16 @@ int ce4b_dequantize_mxfp4(const void* codes_dev, const void* scales_dev, void* o
  * rows (search batches): the time goes to reading the 4-bit weight, once per 64 rows (at most
  * 65535 times). x, codes and scales are 16-byte aligned, k is a multiple of 128. Weights count
  * with the values ce4b_dequantize_mxfp4 gives. A row of x that holds a NaN or an infinity
- * gives a row of non-finite values. */
+ * gives a row of non-finite values. Results repeat bit for bit for the same extents and do not
+ * depend on the other rows' values; the order of the FP32 sums, and with it a rounding, follows
+ * the number of rows. */
 int ce4b_mxfp4_linear(const void* x_dev, const void* codes_dev, const void* scales_dev,
                       const void* residual_dev, void* out_dev, int rows, int n, int k,
                       void* stream);
 
 /* hidden[rows, H] = bf16(silu(g) * u), g and u the products of x [rows, k] with rows 0..H-1
- * and H..2H-1 of an MXFP4 weight [2H, k] (gate rows first; FP32, rounded once at the end). */
+ * and H..2H-1 of an MXFP4 weight [2H, k] (gate rows first; FP32, rounded once at the end; a
+ * gate below -88, whose exponential leaves FP32, gives -0). Sums as in ce4b_mxfp4_linear. */
 int ce4b_mxfp4_swiglu(const void* x_dev, const void* codes_dev, const void* scales_dev,
                       void* hidden_dev, int rows, int hidden_dim, int k, void* stream);
 
