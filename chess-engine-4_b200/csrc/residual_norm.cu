@@ -361,7 +361,7 @@ void launch_norm(const NormArgs& a) {
   const int64_t rows = MX ? (static_cast<int64_t>(a.rows) + 127) / 128 * 128 : a.rows;
   // Blocks that take rows in turn, 2048 threads an SM. The forms for many rows use 54 to 64
   // registers a thread, so that about half of these blocks are on the GPU at once and the others
-  // follow as they leave; a block for every row was slower.
+  // follow as they leave; a block for every row was slower at most sizes.
   const int64_t grid = std::min<int64_t>((rows + kRows - 1) / kRows, static_cast<int64_t>(sm_count()) * (2048 / kThreads));
   launch(add_rmsnorm_kernel<V, TPR, ALIGNED, MX>, dim3(static_cast<unsigned>(grid)), kThreads, 0, 0, a.s,
          a.x, a.residual, a.w, a.sum, a.out, a.codes, a.scales, a.rows, a.width, 1.0 / a.width, a.eps);
